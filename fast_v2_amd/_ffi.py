@@ -105,6 +105,34 @@ class QkvRopeDesc(ctypes.Structure):
     ]
 
 
+class PagePool(ctypes.Structure):
+    """Mirror of ``fdllm_page_pool`` (include/fdllm_hip.h)."""
+
+    _fields_ = [
+        ("page_table", _c_vp), ("table_stride", _c_i64), ("lens", _c_vp), ("free_pages", _c_vp), ("free_count", _c_vp),
+        ("requests", _c_int), ("max_pages", _c_int), ("num_free", _c_int), ("page_size", _c_int),
+    ]
+
+
+class NormRopeKVDesc(ctypes.Structure):
+    """Mirror of ``fdllm_norm_rope_kv_desc`` (include/fdllm_hip.h)."""
+
+    _fields_ = [
+        ("q", _c_vp), ("q_stride_b", _c_i64), ("q_stride_s", _c_i64), ("q_stride_h", _c_i64),
+        ("k", _c_vp), ("k_stride_b", _c_i64), ("k_stride_s", _c_i64), ("k_stride_h", _c_i64),
+        ("v", _c_vp), ("v_stride_b", _c_i64), ("v_stride_s", _c_i64), ("v_stride_h", _c_i64),
+        ("positions", _c_vp), ("inv_freq", _c_vp), ("q_weight", _c_vp), ("k_weight", _c_vp),
+        ("q_out", _c_vp), ("k_out", _c_vp),
+        ("k_cache", _c_vp), ("k_stride_page", _c_i64), ("k_stride_slot", _c_i64), ("k_stride_ch", _c_i64),
+        ("v_cache", _c_vp), ("v_stride_page", _c_i64), ("v_stride_slot", _c_i64), ("v_stride_ch", _c_i64),
+        ("slots", _c_vp), ("num_pages", _c_i64), ("page_size", _c_int),
+        ("batch", _c_int), ("seq_len", _c_int), ("num_q_heads", _c_int), ("num_kv_heads", _c_int),
+        ("head_dim", _c_int), ("rotary_dim", _c_int),
+        ("interleaved", _c_int), ("dtype", _c_int), ("weight_dtype", _c_int),
+        ("eps", _c_float), ("rope_scale", _c_float),
+    ]
+
+
 # name -> (restype, argtypes); every symbol of include/fdllm_hip.h
 SIGNATURES = {
     "fdllm_abi_version": (_c_int, []),
@@ -169,6 +197,20 @@ SIGNATURES = {
         _c_vp, _c_vp, _c_vp,
         _c_int, _c_int, _c_int,
         _c_vp, _c_sz, _c_vp,                    # workspace, bytes, stream
+    ]),
+    "fdllm_assign_pages": (_c_int, [
+        ctypes.POINTER(PagePool), _c_vp, _c_int, _c_int,  # pool, new_lens, width, rows
+        _c_vp, _c_vp, _c_vp, _c_vp,                       # slots, positions, sequences, row_starts
+        _c_vp, _c_vp, _c_vp, _c_vp,                       # starts, seqlens, granted, stream
+    ]),
+    "fdllm_release_pages": (_c_int, [ctypes.POINTER(PagePool), _c_vp, _c_vp]),  # pool, keep_lens, stream
+    "fdllm_norm_rope_kv_write": (_c_int, [ctypes.POINTER(NormRopeKVDesc), _c_vp]),
+    "fdllm_token_logprobs_workspace_size": (_c_int, [_c_int, _c_i64, _c_int, ctypes.POINTER(_c_sz)]),
+    "fdllm_token_logprobs": (_c_int, [
+        _c_vp, _c_i64, _c_i64, _c_int, _c_int, _c_int,  # logits, strides (batch, row), batch, rows, vocab
+        _c_vp, _c_int, _c_int,                          # tokens, given, top
+        _c_vp, _c_vp, _c_vp, _c_vp,                     # logprobs, entropy, top_logprobs, top_tokens
+        _c_int, _c_vp, _c_sz, _c_vp,                    # dtype, workspace, bytes, stream
     ]),
 }
 

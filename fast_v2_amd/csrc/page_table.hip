@@ -1,0 +1,289 @@
+// Pages for a step's new tokens (fdllm_assign_pages) and back (fdllm_release_pages): the page
+// table, slots and positions that the paged cache's callers need, from the requests' lengths,
+// without a word from the host.
+//
+// With page size p, request b's pages in hand h_b = ceil(len_b / p) and after the step
+// t_b = ceil((len_b + n_b) / p), it needs d_b = t_b - h_b pages; with c_b the running sum of d
+// it gets them when c_b is at most the free count, as new page number i = c_b - d_b + (0 ..
+// d_b - 1), which is free_pages[free_count - 1 - i]. Rows of a packed token list begin at the
+// running sum of n. Both sums are one scan over the requests in one workgroup (saturating
+// 32-bit sums of non-negative numbers, which stay associative: what does not fit saturates
+// above every capacity). Because c is monotone, the requests that got pages are a prefix of
+// those that asked, so the request of page i is the first one with c_b > i: a binary search in
+// LDS, which spreads the pages of one long prompt over all threads as evenly as one page each
+// of many requests.
+//
+// What bounds it: latency. The bytes of the largest call take 0.2 us; the calls are chains
+// of dependent memory round trips (lengths, free list or table, stores).
+#include "fdllm_common.h"
+
+namespace fdllm {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kMaxRequests = 8192;
+
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+
+// The sum over the threads before this one, and over all.
+struct Scan {
+  uint32_t before, all;
+};
+__device__ __forceinline__ Scan block_scan(uint32_t x, uint32_t* s_wave) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t up = __shfl_up(x, o, kWave);
+    if (lane >= o) x = add_sat(x, up);
+  }
+  if (lane == 63) s_wave[wave] = x;
+  const uint32_t up = __shfl_up(x, 1, kWave);  // saturated sums do not subtract
+  __syncthreads();
+  Scan r{0, 0};
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w == wave) r.before = add_sat(r.all, lane != 0 ? up : 0);
+    r.all = add_sat(r.all, s_wave[w]);
+  }
+  return r;
+}
+
+// First b < n with upto[b] > i (n if there is none).
+__device__ __forceinline__ int first_above(const uint32_t* upto, int n, uint32_t i) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (upto[mid] > i) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+struct AssignArgs {
+  fdllm_page_pool pool;
+  const int32_t* new_lens;
+  int width, rows, shift;
+  int64_t* slots;
+  int32_t* positions;
+  int32_t* sequences;
+  int32_t* row_starts;
+  int32_t* starts;
+  int32_t* seqlens;
+  int32_t* granted;
+};
+
+// A row's slot and position, given its request's numbers.
+__device__ __forceinline__ void put_row(const AssignArgs& a, int64_t r, int b, bool live, int64_t pos, int64_t slot) {
+  a.slots[r] = slot;
+  a.positions[r] = live ? static_cast<int32_t>(pos) : 0;
+  if (a.sequences) a.sequences[r] = live ? b : -1;
+}
+
+// The requests' part: one workgroup, ITEMS consecutive requests per thread.
+template <int ITEMS>
+__global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignArgs a) {
+  __shared__ uint32_t s_wave[2][kPlanThreads / 64];
+  __shared__ uint32_t s_upto[kPlanThreads * ITEMS];  // running sum of the needs
+  __shared__ int32_t s_at[kPlanThreads * ITEMS];     // table column of page i: s_at + i
+  __shared__ uint32_t s_taken;
+  const fdllm_page_pool& p = a.pool;
+  const int tid = threadIdx.x;
+  const uint32_t avail = static_cast<uint32_t>(min(max(*p.free_count, 0), p.num_free));
+  const uint32_t mask = (1u << a.shift) - 1;
+  if (tid == 0) s_taken = 0;
+  uint32_t n[ITEMS], len[ITEMS], need[ITEMS], have[ITEMS];
+  bool asks[ITEMS];
+  uint32_t sum_n = 0, sum_need = 0;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int b = tid * ITEMS + k;
+    n[k] = b < p.requests ? max(a.new_lens[b], 0) : 0;
+    len[k] = b < p.requests ? max(p.lens[b], 0) : 0;
+    sum_n = add_sat(sum_n, n[k]);
+  }
+  // rows first (their sum does not depend on what is granted), then the needs of those that fit
+  uint32_t at = block_scan(sum_n, s_wave[0]).before;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int b = tid * ITEMS + k;
+    if (a.row_starts && b < p.requests) a.row_starts[b] = static_cast<int32_t>(min(at, 0x7fffffffu));
+    at = add_sat(at, n[k]);
+    if (a.row_starts && b == p.requests - 1) a.row_starts[p.requests] = static_cast<int32_t>(min(at, 0x7fffffffu));
+    // lengths are below 2^31, so their sum fits 32 unsigned bits
+    const uint32_t total = (len[k] + n[k] + mask) >> a.shift;
+    have[k] = (len[k] + mask) >> a.shift;
+    asks[k] = n[k] > 0 && len[k] + n[k] <= 0x7fffffffu && total <= static_cast<uint32_t>(p.max_pages) &&
+              (a.width > 0 ? n[k] <= static_cast<uint32_t>(a.width) : at <= static_cast<uint32_t>(a.rows));
+    need[k] = asks[k] ? total - have[k] : 0;
+    sum_need = add_sat(sum_need, need[k]);
+  }
+  uint32_t c = block_scan(sum_need, s_wave[1]).before;
+  uint32_t taken = 0;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int b = tid * ITEMS + k;
+    s_at[b] = static_cast<int32_t>(have[k] - c);
+    c = add_sat(c, need[k]);
+    s_upto[b] = c;
+    const bool ok = asks[k] && (need[k] == 0 || c <= avail);
+    if (ok) taken = max(taken, need[k] ? c : 0);
+    if (b < p.requests) {
+      const int32_t old = p.lens[b];
+      const uint32_t got = ok ? n[k] : 0;
+      a.starts[b] = static_cast<int32_t>(len[k]);
+      a.seqlens[b] = static_cast<int32_t>(len[k] + got);
+      a.granted[b] = static_cast<int32_t>(got);
+      if (ok) p.lens[b] = static_cast<int32_t>(len[k] + got);
+      else if (old < 0) p.lens[b] = 0;
+    }
+  }
+  if (taken) atomicMax(&s_taken, taken);
+  __syncthreads();
+  taken = s_taken;
+  for (uint32_t i = tid; i < taken; i += kPlanThreads) {
+    const int b = first_above(s_upto, p.requests, i);
+    p.page_table[b * p.table_stride + static_cast<int32_t>(s_at[b] + i)] = p.free_pages[avail - 1 - i];
+  }
+  if (tid == 0) *p.free_count = static_cast<int32_t>(avail - taken);
+}
+
+// The rows' part, after the plan.
+__global__ __launch_bounds__(256) void assign_rows_kernel(const AssignArgs a, int64_t n_rows) {
+  const fdllm_page_pool& p = a.pool;
+  for (int64_t r = blockIdx.x * 256ll + threadIdx.x; r < n_rows; r += gridDim.x * 256ll) {
+    int b, t;
+    bool live;
+    if (a.width > 0) {
+      b = static_cast<int>(r / a.width);
+      t = static_cast<int>(r - static_cast<int64_t>(b) * a.width);
+      live = t < a.new_lens[b];
+    } else {
+      // the last request that begins at or before r and is not empty: the first whose end is above r
+      b = first_above(reinterpret_cast<const uint32_t*>(a.row_starts + 1), p.requests, static_cast<uint32_t>(r));
+      live = b < p.requests;
+      t = live ? static_cast<int>(r) - a.row_starts[b] : 0;
+    }
+    int64_t pos = 0, slot = -1;
+    if (live) {
+      pos = static_cast<int64_t>(a.starts[b]) + t;
+      if (a.granted[b] > 0)
+        slot = (static_cast<int64_t>(p.page_table[b * p.table_stride + (pos >> a.shift)]) << a.shift) +
+               (pos & ((1 << a.shift) - 1));
+    }
+    put_row(a, r, b, live, pos, slot);
+  }
+}
+
+// keep_lens: pages behind the kept lengths go back, the last ones first.
+struct ReleaseArgs {
+  fdllm_page_pool pool;
+  const int32_t* keep_lens;
+  int shift;
+};
+
+template <int ITEMS>
+__global__ __launch_bounds__(kPlanThreads) void release_kernel(const ReleaseArgs a) {
+  __shared__ uint32_t s_wave[kPlanThreads / 64];
+  __shared__ uint32_t s_upto[kPlanThreads * ITEMS];
+  __shared__ int32_t s_at[kPlanThreads * ITEMS];
+  const fdllm_page_pool& p = a.pool;
+  const int tid = threadIdx.x;
+  const uint32_t count = static_cast<uint32_t>(min(max(*p.free_count, 0), p.num_free));
+  const uint32_t mask = (1u << a.shift) - 1;
+  uint32_t kept[ITEMS], back[ITEMS], sum = 0;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int b = tid * ITEMS + k;
+    kept[k] = back[k] = 0;
+    if (b < p.requests) {
+      const uint32_t len = max(p.lens[b], 0);
+      const uint32_t keep = min(static_cast<uint32_t>(max(a.keep_lens[b], 0)), len);
+      const uint32_t most = static_cast<uint32_t>(p.max_pages);
+      kept[k] = min((keep + mask) >> a.shift, most);
+      back[k] = min((len + mask) >> a.shift, most) - kept[k];
+      p.lens[b] = static_cast<int32_t>(keep);
+    }
+    sum = add_sat(sum, back[k]);
+  }
+  const Scan scan = block_scan(sum, s_wave);
+  uint32_t c = scan.before;
+  const uint32_t n = min(scan.all, static_cast<uint32_t>(p.num_free) - count);
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    s_at[tid * ITEMS + k] = static_cast<int32_t>(kept[k] - c);
+    c = add_sat(c, back[k]);
+    s_upto[tid * ITEMS + k] = c;
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < n; i += kPlanThreads) {
+    const int b = first_above(s_upto, p.requests, i);
+    p.free_pages[count + n - 1 - i] = p.page_table[b * p.table_stride + static_cast<int32_t>(s_at[b] + i)];
+  }
+  if (tid == 0) *p.free_count = static_cast<int32_t>(count + n);
+}
+
+int check_pool(const char* what, const fdllm_page_pool* p) {
+  FDLLM_CHECK_ARG(p != nullptr, "%s: null pool", what);
+  FDLLM_CHECK_ARG(p->requests >= 0 && p->requests <= kMaxRequests, "%s: %d requests (0 to %d)", what, p->requests,
+                  kMaxRequests);
+  FDLLM_CHECK_ARG(p->page_size > 0 && (p->page_size & (p->page_size - 1)) == 0,
+                  "%s: page_size %d is not a power of two", what, p->page_size);
+  FDLLM_CHECK_ARG(p->max_pages >= 0 && p->num_free >= 0 && p->table_stride >= p->max_pages,
+                  "%s: bad table or free list size", what);
+  if (p->requests == 0) return FDLLM_OK;
+  FDLLM_CHECK_ARG((p->page_table || p->max_pages == 0) && p->lens && (p->free_pages || p->num_free == 0) && p->free_count,
+                  "%s: null pointer", what);
+  return FDLLM_OK;
+}
+
+}  // namespace
+}  // namespace fdllm
+
+extern "C" int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* new_lens, int width, int rows,
+                                  int64_t* slots, int32_t* positions, int32_t* sequences, int32_t* row_starts,
+                                  int32_t* starts, int32_t* seqlens, int32_t* granted, void* stream) {
+  using namespace fdllm;
+  const char* what = "fdllm_assign_pages";
+  if (const int rc = check_pool(what, pool)) return rc;
+  FDLLM_CHECK_ARG(width >= 0 && rows >= 0 && (width == 0 || rows == 0),
+                  "%s: give the padded form's width or the packed form's rows", what);
+  if (pool->requests == 0 && (width > 0 || rows == 0)) return FDLLM_OK;
+  FDLLM_CHECK_ARG(pool->requests > 0, "%s: a packed list without requests", what);
+  FDLLM_CHECK_ARG(new_lens && slots && positions && starts && seqlens && granted && (width > 0 || (sequences && row_starts)),
+                  "%s: null pointer", what);
+  AssignArgs a;
+  a.pool = *pool;
+  a.new_lens = new_lens;
+  a.width = width;
+  a.rows = rows;
+  a.shift = __builtin_ctz(static_cast<unsigned>(pool->page_size));
+  a.slots = slots;
+  a.positions = positions;
+  a.sequences = width > 0 ? nullptr : sequences;
+  a.row_starts = width > 0 ? nullptr : row_starts;
+  a.starts = starts;
+  a.seqlens = seqlens;
+  a.granted = granted;
+  const int64_t n_rows = width > 0 ? static_cast<int64_t>(width) * pool->requests : rows;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (pool->requests <= kPlanThreads) assign_plan_kernel<1><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
+  else assign_plan_kernel<kMaxRequests / kPlanThreads><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
+  if (n_rows > 0) {
+    const int64_t wgs = (n_rows + 255) / 256;
+    assign_rows_kernel<<<dim3(static_cast<unsigned>(wgs < 2048 ? wgs : 2048)), dim3(256), 0, s>>>(a, n_rows);
+  }
+  FDLLM_RETURN_LAUNCH_STATUS(what);
+}
+
+extern "C" int fdllm_release_pages(const fdllm_page_pool* pool, const int32_t* keep_lens, void* stream) {
+  using namespace fdllm;
+  const char* what = "fdllm_release_pages";
+  if (const int rc = check_pool(what, pool)) return rc;
+  if (pool->requests == 0) return FDLLM_OK;
+  FDLLM_CHECK_ARG(keep_lens != nullptr, "%s: null pointer", what);
+  ReleaseArgs a{*pool, keep_lens, __builtin_ctz(static_cast<unsigned>(pool->page_size))};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (pool->requests <= kPlanThreads) release_kernel<1><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
+  else release_kernel<kMaxRequests / kPlanThreads><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
+  FDLLM_RETURN_LAUNCH_STATUS(what);
+}

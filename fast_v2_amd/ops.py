@@ -22,12 +22,13 @@ in the manner of ``_wrap_flash_kvcache_as_custom_op``
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import logging
 import math
 import threading
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
@@ -885,6 +886,319 @@ def kv_cache_write(
         _ptr(write_start), int(write_offset), _ptr(positions),
         B, T, Hkv, D, _ffi.dtype_code(k_new.dtype), _ffi.stream_ptr(dev))
     _ffi.check(rc, "fdllm_kv_cache_write")
+
+
+# ---------------------------------------------------------------------------
+# around the paged cache: pages for new tokens, head norms + rotation + paged write, scores
+# ---------------------------------------------------------------------------
+
+_INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+def _no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Inference calls: a tensor to differentiate is refused, its gradient would be lost."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: no backward pass (call it under torch.no_grad(), or detach the tensors)")
+
+
+def _launching(dev: torch.device):
+    """Makes ``dev`` the current device of a launch (the null stream is the current device's)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _int32(what: str, t: torch.Tensor) -> torch.Tensor:
+    """Contiguous int32 values; larger ones of other integer types are held at its limits."""
+    if t.dtype not in _INTS:
+        raise RuntimeError(f"{what}: integers expected, got {t.dtype}")
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(torch.int32).contiguous()
+
+
+class PageRows(NamedTuple):
+    """What ``assign_pages`` says of a step's rows ([requests, width], or [rows] in the packed
+    form) and of its requests."""
+
+    slots: torch.Tensor                # int64: page * page_size + offset, -1 where there is none
+    positions: torch.Tensor            # int32
+    starts: torch.Tensor               # int32 [requests]: lengths before the step
+    seqlens: torch.Tensor              # int32 [requests]: and after it
+    granted: torch.Tensor              # int32 [requests]: new tokens that got their slots
+    sequences: Optional[torch.Tensor]  # packed: int32 [rows], the request of a row or -1
+    row_starts: Optional[torch.Tensor]  # packed: int32 [requests + 1], where a request's rows begin
+
+
+def _page_pool(what, lens, page_table, free_pages, free_count, page_size, *more):
+    dev = _require_gpu(lens, page_table, free_pages, free_count, *more)
+    if any(t.dtype != torch.int32 for t in (lens, page_table, free_pages, free_count)):
+        raise RuntimeError(f"{what}: lens, page_table, free_pages and free_count must be int32 (changed in place)")
+    if page_table.dim() != 2 or lens.shape != page_table.shape[:1] or free_pages.dim() != 1 or free_count.numel() != 1:
+        raise RuntimeError(f"{what}: expected lens [B], page_table [B, max_pages], free_pages [F], free_count [1]")
+    if not (lens.is_contiguous() and free_pages.is_contiguous()) or (page_table.numel() and page_table.stride(1) != 1):
+        raise RuntimeError(f"{what}: lens, free_pages and the page table's rows must be contiguous")
+    if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
+        raise RuntimeError(f"{what}: page_table rows overlap")
+    p = _ffi.PagePool()
+    p.page_table, p.table_stride = page_table.data_ptr(), max(page_table.stride(0), page_table.shape[1])
+    p.lens, p.free_pages, p.free_count = lens.data_ptr(), free_pages.data_ptr(), free_count.data_ptr()
+    p.requests, p.max_pages = page_table.shape
+    p.num_free, p.page_size = free_pages.numel(), int(page_size)
+    return p, dev
+
+
+def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, page_size: int, width: int = 0, rows: int = 0) -> PageRows:
+    """Pages, slots and positions for a step's new tokens, from the requests' lengths on the GPU.
+
+    new_lens   [B] tokens that each request asks for (int32; other ints converted)
+    lens       [B] int32 tokens in each request's cache; grows by what is granted
+    page_table [B, max_pages] int32, ``block_attn``'s; new pages are entered
+    free_pages [F] int32 page ids, the first ``free_count`` [1] int32 of them free; the last
+               one is handed out first
+    width      padded form: row (b, t) of [B, width] is request b's t-th new token, or
+    rows       packed form: the requests' rows one after another in a list of ``rows``
+
+    A request gets all of its tokens or none (``granted``): none if its table row, ``width`` or
+    ``rows`` cannot hold them, or if the pages have run out; after the first one that found too
+    few pages, only requests with room on their last page are served. ``slots`` and
+    ``positions`` go to ``norm_rope_kv_write``, ``seqlens`` (and ``starts`` as ``q_start``) with
+    the table to ``block_attn``. page_size is a power of two; at most 8192 requests. Changes
+    ``lens``, ``page_table`` and ``free_count`` in place: calls on one pool run in stream order.
+    """
+    what = "assign_pages"
+    if (width > 0) == (rows > 0) or width < 0 or rows < 0:
+        raise RuntimeError(f"{what}: give the padded form's width or the packed form's rows")
+    p, dev = _page_pool(what, lens, page_table, free_pages, free_count, page_size, new_lens)
+    if new_lens.shape != lens.shape:
+        raise RuntimeError(f"{what}: new_lens must be [B]")
+    new_lens = _int32(what, new_lens)
+    B = p.requests
+    shape = (B, width) if width else (rows,)
+    slots = torch.empty(shape, dtype=torch.int64, device=dev)
+    positions = torch.empty(shape, dtype=torch.int32, device=dev)
+    starts, seqlens, granted = (torch.empty(B, dtype=torch.int32, device=dev) for _ in range(3))
+    sequences = row_starts = None
+    if not width:
+        sequences = torch.empty(rows, dtype=torch.int32, device=dev)
+        row_starts = torch.empty(B + 1, dtype=torch.int32, device=dev)
+    with _launching(dev):
+        rc = _ffi.lib().fdllm_assign_pages(
+            ctypes.byref(p), new_lens.data_ptr(), int(width), int(rows), slots.data_ptr(), positions.data_ptr(),
+            _ptr(sequences), _ptr(row_starts), starts.data_ptr(), seqlens.data_ptr(), granted.data_ptr(),
+            _ffi.stream_ptr(dev))
+    _ffi.check(rc, "fdllm_assign_pages")
+    return PageRows(slots, positions, starts, seqlens, granted, sequences, row_starts)
+
+
+def release_pages(keep_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, page_size: int) -> None:
+    """Cuts each request's cache to ``keep_lens`` [B] tokens (no change where it is shorter; 0
+    ends a request) and gives the pages behind back to the free list, in the reverse of
+    ``assign_pages``' order: releasing a whole step leaves the pool as it was before it."""
+    what = "release_pages"
+    p, dev = _page_pool(what, lens, page_table, free_pages, free_count, page_size, keep_lens)
+    if keep_lens.shape != lens.shape:
+        raise RuntimeError(f"{what}: keep_lens must be [B]")
+    keep_lens = _int32(what, keep_lens)
+    with _launching(dev):
+        rc = _ffi.lib().fdllm_release_pages(ctypes.byref(p), keep_lens.data_ptr(), _ffi.stream_ptr(dev))
+    _ffi.check(rc, "fdllm_release_pages")
+
+
+def rope_frequencies(rotary_dim: int, base: float = 1e6, scaling: Optional[str] = None, factor: float = 1.0,
+                     original_len: int = 4096, device=None) -> Tuple[torch.Tensor, float]:
+    """(inv_freq [rotary_dim / 2] fp32, rope_scale) for ``norm_rope_kv_write``: f_i = base^(-2 i /
+    rotary_dim), stretched to contexts ``factor`` times ``original_len``:
+
+      None      as they are
+      "linear"  f / factor (position interpolation, Chen et al. 2023)
+      "ntk"     base * factor^(d / (d - 2)): the slowest one by factor, the fastest not at all
+      "yarn"    f / factor where f makes at most 1 turn over original_len, f where it makes at
+                least 32, a ramp between; rope_scale = 0.1 ln(factor) + 1 (Peng et al. 2023)
+    """
+    if rotary_dim < 0 or rotary_dim % 2 or base <= 0 or factor <= 0:
+        raise RuntimeError("rope_frequencies: rotary_dim must be even, base and factor positive")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise RuntimeError(f"rope_frequencies: unknown scaling {scaling!r}")
+    if scaling == "ntk":
+        if rotary_dim < 4:
+            raise RuntimeError("rope_frequencies: ntk scaling needs at least 4 rotary dimensions")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    f = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / max(rotary_dim, 1))
+    scale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        turns = original_len * f / (2 * math.pi)
+        keep = ((turns - 1.0) / 31.0).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        scale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    return f.to(device=device, dtype=torch.float32), scale
+
+
+def norm_rope_kv_write(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    inv_freq: torch.Tensor,
+    q_weight: Optional[torch.Tensor] = None,
+    k_weight: Optional[torch.Tensor] = None,
+    eps: float = 1e-6,
+    k_cache: Optional[torch.Tensor] = None,
+    v_cache: Optional[torch.Tensor] = None,
+    slots: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    rope_scale: float = 1.0,
+    kv_out: bool = False,
+):
+    """RMSNorm of every query and key head, the position rotation, and the K / V rows' write
+    into a page pool, in one kernel.
+
+    q          [B, S, Hq, D], k / v [B, S, Hkv, D] bf16, fp16 or fp32 (a packed token list is
+               B = 1); D a multiple of 8, at most 256
+    positions  [B, S] of the tokens (int32; other ints converted)
+    inv_freq   [R / 2] fp32, R even, at most D: dimensions from R on are not rotated
+               (``rope_frequencies`` makes it; rope_scale multiplies cos and sin)
+    q_weight, k_weight  [D] of the norms (the heads' dtype or fp32); None: that one is not normed
+    k_cache, v_cache    [num_pages, page_size, Hkv, D] pools in any strides of whole 16-byte
+               rows (``block_attn``'s); written in place at ``slots`` [B, S] (page * page_size +
+               offset; rows outside of the pool, as -1, are not written; repeated slots race)
+    interleaved  pairs are (2 i, 2 i + 1) in place of (i, i + R / 2)
+
+    Held in fp32 (angles in 64 bits) and rounded once. Returns the new queries [B, S, Hq, D],
+    with kv_out=True also the new keys [B, S, Hkv, D]. page_size is a power of two.
+    """
+    what = "norm_rope_kv_write"
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise RuntimeError(f"{what}: q [B, S, Hq, D], k / v [B, S, Hkv, D] expected")
+    B, S, Hq, D = q.shape
+    Hkv = k.shape[2]
+    if (k_cache is None) != (v_cache is None) or (k_cache is None) != (slots is None):
+        raise RuntimeError(f"{what}: give k_cache, v_cache and slots together")
+    given = [t for t in (positions, inv_freq, q_weight, k_weight, k_cache, v_cache, slots) if t is not None]
+    dev = _require_gpu(q, k, v, *given)
+    _no_grad(what, q, k, v, inv_freq, q_weight, k_weight, k_cache, v_cache)
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32) or \
+            any(t is not None and t.dtype != q.dtype for t in (k, v, k_cache, v_cache)):
+        raise RuntimeError(f"{what}: q, k, v and the caches must share bf16, fp16 or fp32")
+    if positions.shape != (B, S) or (slots is not None and slots.shape != (B, S)):
+        raise RuntimeError(f"{what}: positions and slots must be [B, S]")
+    if inv_freq.dim() != 1 or not inv_freq.is_floating_point() or 2 * inv_freq.numel() > D:
+        raise RuntimeError(f"{what}: inv_freq must be floating [R / 2] with R at most head_dim")
+    weights = [q_weight, k_weight]
+    for w in weights:
+        if w is not None and (w.shape != (D,) or w.dtype not in (q.dtype, torch.float32)):
+            raise RuntimeError(f"{what}: norm weights must be [head_dim] in the heads' dtype or fp32")
+    if len({w.dtype for w in weights if w is not None}) > 1:
+        weights = [w.float() for w in weights]
+    vec = 16 // q.element_size()
+
+    def rows(t):  # 16-byte rows
+        return t.stride(-1) == 1 and all(st % vec == 0 for st in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+
+    def aligned(t):
+        if t is None or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0):
+            return t
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    q, k, v = (t if rows(t) else t.contiguous() if not t.is_contiguous() else t.clone() for t in (q, k, v))
+    weights = [aligned(w) for w in weights]
+    positions, inv_freq = _int32(what, positions), inv_freq.float().contiguous()
+    q_out = torch.empty((B, S, Hq, D), dtype=q.dtype, device=dev)
+    k_out = torch.empty((B, S, Hkv, D), dtype=q.dtype, device=dev) if kv_out else None
+    d = _ffi.NormRopeKVDesc()
+    if k_cache is not None:
+        if slots.dtype not in _INTS:
+            raise RuntimeError(f"{what}: slots must be integers, got {slots.dtype}")
+        slots = slots.to(torch.int64).contiguous()
+        for c in (k_cache, v_cache):
+            if c.dim() != 4 or c.shape[2:] != (Hkv, D) or c.shape != k_cache.shape:
+                raise RuntimeError(f"{what}: caches must be [num_pages, page_size, Hkv, D]")
+            if not rows(c) or any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
+                raise RuntimeError(f"{what}: cache rows must be contiguous, apart and 16-byte aligned (written in place)")
+        d.k_cache, (d.k_stride_page, d.k_stride_slot, d.k_stride_ch) = k_cache.data_ptr(), k_cache.stride()[:3]
+        d.v_cache, (d.v_stride_page, d.v_stride_slot, d.v_stride_ch) = v_cache.data_ptr(), v_cache.stride()[:3]
+        d.slots, d.num_pages, d.page_size = slots.data_ptr(), k_cache.shape[0], k_cache.shape[1]
+    d.q, (d.q_stride_b, d.q_stride_s, d.q_stride_h) = q.data_ptr(), q.stride()[:3]
+    d.k, (d.k_stride_b, d.k_stride_s, d.k_stride_h) = k.data_ptr(), k.stride()[:3]
+    d.v, (d.v_stride_b, d.v_stride_s, d.v_stride_h) = v.data_ptr(), v.stride()[:3]
+    d.positions, d.inv_freq = positions.data_ptr(), inv_freq.data_ptr()
+    d.q_weight, d.k_weight = _ptr(weights[0]), _ptr(weights[1])
+    d.q_out, d.k_out = q_out.data_ptr(), _ptr(k_out)
+    d.batch, d.seq_len, d.num_q_heads, d.num_kv_heads, d.head_dim = B, S, Hq, Hkv, D
+    d.rotary_dim, d.interleaved, d.dtype = 2 * inv_freq.numel(), int(bool(interleaved)), _ffi.dtype_code(q.dtype)
+    d.weight_dtype = next((_ffi.dtype_code(w.dtype) for w in weights if w is not None), d.dtype)
+    d.eps, d.rope_scale = float(eps), float(rope_scale)
+    with _launching(dev):
+        rc = _ffi.lib().fdllm_norm_rope_kv_write(ctypes.byref(d), _ffi.stream_ptr(dev))
+    _ffi.check(rc, "fdllm_norm_rope_kv_write")
+    return (q_out, k_out) if kv_out else q_out
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` says of every row, in fp32."""
+
+    logprobs: Optional[torch.Tensor]      # of the given tokens, in their shape
+    entropy: torch.Tensor                 # [...]
+    top_logprobs: Optional[torch.Tensor]  # [..., top_k]
+    top_tokens: Optional[torch.Tensor]    # int64 [..., top_k]
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprobs_bytes(vocab: int, rows: int, dtype: int) -> int:
+    need = ctypes.c_size_t(0)
+    _ffi.check(_ffi.lib().fdllm_token_logprobs_workspace_size(vocab, rows, dtype, ctypes.byref(need)),
+               "fdllm_token_logprobs_workspace_size")
+    return need.value
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens, the entropy and the ``top_k`` most probable tokens of
+    every row of logits, in one pass over them.
+
+    logits  [..., V] bf16, fp16 or fp32; rows of any alignment, up to three dimensions in any
+            strides (a shifted view of a text's logits is read in place)
+    tokens  [...] or [..., M] ids of each row (int64; other ints converted), or None
+    top_k   at most 32
+
+    Equal logits count in the order of their ids. Ids outside of the vocabulary get NaN; rows
+    without a distribution (NaN, +inf, or nothing above -inf) NaN and top_tokens of -1. Scratch
+    is allocated by the call, so calls on several streams and captured ones are apart.
+    """
+    what = "token_logprobs"
+    if logits.dim() < 1 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise RuntimeError(f"{what}: logits [..., V] in bf16, fp16 or fp32 expected")
+    dev = _require_gpu(logits, *([tokens] if tokens is not None else []))
+    _no_grad(what, logits)
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(32, V):
+        raise RuntimeError(f"{what}: top_k {top_k} must be at most 32 and the vocabulary's size")
+    given = 0
+    if tokens is not None:
+        if tokens.dtype not in _INTS or (tokens.shape != lead and tokens.shape[:-1] != lead):
+            raise RuntimeError(f"{what}: integer tokens {tuple(lead)} or {tuple(lead)} + (M,) expected")
+        given = 1 if tokens.shape == lead else tokens.shape[-1]
+        tokens = tokens.to(torch.int64).contiguous()
+    if V and logits.stride(-1) != 1:
+        logits = logits.contiguous()
+    x = logits if logits.dim() <= 3 else logits.reshape(-1, V)
+    batch, rows = (1, 1) if x.dim() == 1 else (1, x.shape[0]) if x.dim() == 2 else x.shape[:2]
+    stride_b, stride_r = (0, 0) if x.dim() == 1 else (0, x.stride(0)) if x.dim() == 2 else x.stride()[:2]
+    f32 = dict(dtype=torch.float32, device=dev)
+    logprobs = torch.empty(tokens.shape, **f32) if tokens is not None else None
+    entropy = torch.empty(lead, **f32)
+    top_logprobs = torch.empty((*lead, top_k), **f32) if top_k else None
+    top_tokens = torch.empty((*lead, top_k), dtype=torch.int64, device=dev) if top_k else None
+    code = _ffi.dtype_code(x.dtype)
+    need = _logprobs_bytes(V, batch * rows, code)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _launching(dev):
+        rc = _ffi.lib().fdllm_token_logprobs(
+            x.data_ptr(), stride_b, stride_r, batch, rows, V, _ptr(tokens), given, top_k, _ptr(logprobs),
+            entropy.data_ptr(), _ptr(top_logprobs), _ptr(top_tokens), code, _ptr(ws), need, _ffi.stream_ptr(dev))
+    _ffi.check(rc, "fdllm_token_logprobs")
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_tokens)
 
 
 # ---------------------------------------------------------------------------

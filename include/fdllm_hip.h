@@ -489,6 +489,129 @@ int fdllm_unmask_step_ws(const void* logits, int64_t logits_stride_b, int64_t lo
                          int batch, int num_positions, int dtype, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* -------------------------------------------------------------------------
+ * Pages for a step's new tokens, from the requests' lengths on the device.
+ *
+ * The pool: page_table [requests, max_pages] (row stride table_stride), lens [requests] (the
+ * tokens in each request's cache; negative counts as 0), and the free list: page ids
+ * free_pages[0 .. *free_count), of which the last is handed out first. page_size is a power of
+ * two (fdllm_kv_attn_fwd takes 16 and more). All int32. The calls below change the pool in
+ * place, in stream order; calls on one pool must not overlap.
+ *
+ * fdllm_assign_pages: request b asks for new_lens[b] tokens (none where it is not positive).
+ *   Its rows: width > 0 (padded form): rows b * width .. + width - 1 of [requests, width];
+ *     width 0 (packed form): from the sum of the requests' new_lens before it, of `rows` in all.
+ *   It is granted all of them or none. None if its table row cannot hold its pages, its rows
+ *   do not fit (more than width, or past the last of `rows`), or if it needs pages and they
+ *   have run out: pages go to the requests in order, and after the first that gets none for
+ *   want of pages no later one gets any (those with room on their last page are granted).
+ *   The new pages, in the order of requests and of columns, are the last of the free list,
+ *   last first. Then lens[b] += granted[b].
+ *   slots[row] = page * page_size + offset for granted tokens, else -1; positions[row] =
+ *   position of the asked token, 0 for rows without one; packed form only: sequences[row] = b
+ *   or -1, row_starts[requests + 1] the rows' prefix sums (at most INT32_MAX). Per request:
+ *   starts (lens before), seqlens (lens after), granted.
+ *   sequences and row_starts are NULL in the padded form. Table columns of pages that were not
+ *   handed out keep what they hold.
+ *
+ * fdllm_release_pages: lens[b] becomes min(lens[b], max(keep_lens[b], 0)); pages behind it go
+ *   back to the free list, in the reverse of the order in which fdllm_assign_pages hands them
+ *   out, so that releasing a whole step restores the list. The table keeps its entries.
+ *
+ * At most 8192 requests. One or two kernels each. No counterpart in the reference, whose page
+ * table is the identity (utils/attention_backends.py:505-510).
+ * ------------------------------------------------------------------------- */
+typedef struct fdllm_page_pool {
+  int32_t* page_table;
+  int64_t table_stride;
+  int32_t* lens;
+  int32_t* free_pages;
+  int32_t* free_count;
+  int requests, max_pages, num_free, page_size; /* num_free: entries that free_pages can hold */
+} fdllm_page_pool;
+
+int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* new_lens, int width, int rows, int64_t* slots,
+                       int32_t* positions, int32_t* sequences, int32_t* row_starts, int32_t* starts,
+                       int32_t* seqlens, int32_t* granted, void* stream);
+int fdllm_release_pages(const fdllm_page_pool* pool, const int32_t* keep_lens, void* stream);
+
+/* -------------------------------------------------------------------------
+ * Norms of the query and key heads, the position rotation and the K / V write into pages.
+ *
+ *   for every token (b, t), query head and key head x[0 .. head_dim):
+ *     x^ = x * rsqrt(mean(x^2) + eps) * weight        (weight NULL: x^ = x)
+ *     a_i = positions[b, t] * inv_freq[i]             (i < rotary_dim / 2, in 64 bits)
+ *     c_i, s_i = rope_scale * cos(a_i), rope_scale * sin(a_i)
+ *     (x0, x1) = x^ at (i, i + rotary_dim / 2), or at (2 i, 2 i + 1) with `interleaved`
+ *     y0 = x0 c_i - x1 s_i,  y1 = x1 c_i + x0 s_i;    y = x^ from rotary_dim on
+ *   held in fp32 and rounded once to `dtype`. q_out[b, t, h] = y; the key rows y and the value
+ *   rows go to slots[b, t] of the pools: page slot / page_size, row slot % page_size. Rows with a
+ *   slot outside of the pool (-1) are not written. Slots that repeat race. k_out (optional,
+ *   [batch, seq_len, num_kv_heads, head_dim] contiguous) also gets the key rows. Without
+ *   k_cache / v_cache / slots (all NULL) no pool is written and v is not read.
+ *
+ * positions, slots: [batch, seq_len] contiguous, int32 and int64. head_dim is a multiple of 8,
+ * at most 256; rotary_dim even, at most head_dim. Rows and strides are multiples of 16 bytes.
+ * q_out is contiguous. weight_dtype: the heads' dtype, or FDLLM_DTYPE_F32. No output may
+ * overlap an input.
+ *
+ * Replaces, for paged caches: _apply_rotary_pos_emb + write_scratch_compiled
+ * (utils/attention_backends.py:777-788; static_kv_cache.py:218-229), with angles from
+ * the positions in place of 16-bit cos / sin rows.
+ * ------------------------------------------------------------------------- */
+typedef struct fdllm_norm_rope_kv_desc {
+  const void* q; /* [batch, seq_len, num_q_heads, head_dim] */
+  int64_t q_stride_b, q_stride_s, q_stride_h;
+  const void* k; /* [batch, seq_len, num_kv_heads, head_dim] */
+  int64_t k_stride_b, k_stride_s, k_stride_h;
+  const void* v;
+  int64_t v_stride_b, v_stride_s, v_stride_h;
+  const int32_t* positions;
+  const float* inv_freq; /* [rotary_dim / 2] */
+  const void* q_weight;  /* [head_dim] or NULL */
+  const void* k_weight;
+  void* q_out;
+  void* k_out; /* or NULL */
+  void* k_cache; /* [num_pages, page_size, num_kv_heads, head_dim] */
+  int64_t k_stride_page, k_stride_slot, k_stride_ch;
+  void* v_cache;
+  int64_t v_stride_page, v_stride_slot, v_stride_ch;
+  const int64_t* slots;
+  int64_t num_pages;
+  int page_size;
+  int batch, seq_len, num_q_heads, num_kv_heads, head_dim, rotary_dim;
+  int interleaved, dtype, weight_dtype;
+  float eps, rope_scale;
+} fdllm_norm_rope_kv_desc;
+
+int fdllm_norm_rope_kv_write(const fdllm_norm_rope_kv_desc* desc, void* stream);
+
+/* -------------------------------------------------------------------------
+ * Log probabilities of given tokens, the entropy and the most probable alternatives of logits
+ * rows (b, r), b < batch, r < rows_per_batch, at logits + b * stride_b + r * stride_r (elements;
+ * any alignment), `vocab` logits each:
+ *
+ *   logprobs[row, j]  = log softmax(row)[tokens[row, j]]     j < given (NaN for ids outside of the vocabulary)
+ *   entropy[row]      = -sum p log p                         (a logit of -inf adds 0)
+ *   top_tokens[row, k], top_logprobs[row, k]                 k < top (at most 32): the largest
+ *     logits, equal ones by their index, and their log probabilities
+ *
+ * in fp32; all outputs contiguous. A row without a distribution (it holds NaN or +inf, or
+ * nothing above -inf) gives NaN, and -1 for top_tokens.
+ *
+ * `workspace` (fdllm_token_logprobs_workspace_size bytes, 0 for many rows; 16-byte aligned)
+ * needs no initialisation; calls that may overlap in time need separate ones. One kernel, or two
+ * where workgroups share a row. vocab is at most 2^22 - 8.
+ *
+ * No counterpart in the reference, whose sampling takes the probability of the greedy token
+ * (modeling.py:2263-2270); for scoring given texts.
+ * ------------------------------------------------------------------------- */
+int fdllm_token_logprobs_workspace_size(int vocab, int64_t rows, int dtype, size_t* bytes);
+int fdllm_token_logprobs(const void* logits, int64_t stride_b, int64_t stride_r, int batch, int rows_per_batch,
+                         int vocab, const int64_t* tokens, int given, int top, float* logprobs, float* entropy,
+                         float* top_logprobs, int64_t* top_tokens, int dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
