@@ -282,7 +282,8 @@ HOST_PATH = Path(__file__).resolve().parent / "lib" / "fdllm_host.so"
 _HOST_APIS = ("fdllm_last_error", "fdllm_kv_attn_workspace_size", "fdllm_kv_attn_fwd", "fdllm_gather_rmsnorm",
               "fdllm_scatter_rows", "fdllm_add_rmsnorm", "fdllm_qkv_rope_workspace_size",
               "fdllm_qkv_rope_kv_write_ws", "fdllm_linear_workspace_size", "fdllm_linear",
-              "fdllm_unmask_workspace_size", "fdllm_unmask_step_ws")
+              "fdllm_unmask_workspace_size", "fdllm_unmask_step_ws", "fdllm_assign_pages", "fdllm_release_pages",
+              "fdllm_norm_rope_kv_write", "fdllm_token_logprobs_workspace_size", "fdllm_token_logprobs")
 
 
 def host_calls(buffers: dict, get):

@@ -1,4 +1,4 @@
-// The host side of the calls that a sub-block step makes, in native code: checks, output
+// The host side of the calls that a step makes, in native code: checks, output
 // allocation, descriptor, workspace lookup and launch of one call of libfdllm_hip.so.
 //
 // Each function takes the tensors of its ops.py namesake and returns its result, or None
@@ -13,12 +13,14 @@
 // its `get` called where a buffer is missing or too small.
 #include <Python.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <initializer_list>
 
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -42,8 +44,13 @@ struct Api {
   decltype(&fdllm_linear) linear;
   decltype(&fdllm_unmask_workspace_size) unmask_size;
   decltype(&fdllm_unmask_step_ws) unmask;
+  decltype(&fdllm_assign_pages) assign;
+  decltype(&fdllm_release_pages) release;
+  decltype(&fdllm_norm_rope_kv_write) norm_rope;
+  decltype(&fdllm_token_logprobs_workspace_size) logprobs_size;
+  decltype(&fdllm_token_logprobs) logprobs;
 } api;
-constexpr int kApis = 12;
+constexpr int kApis = 17;
 
 PyObject* g_stream = nullptr;   // torch's raw stream lookup: device index -> handle
 PyObject* g_buffers = nullptr;  // ops._Workspace's dictionary: (device index, stream) -> tensor
@@ -502,6 +509,214 @@ PyObject* unmask(PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
+// The calls below make their device current for the launch; here it has to be already.
+void on_current_device(const Tensor& t) {
+  plain(t.device().index() == c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice().index());
+}
+
+bool whole_ints(const Tensor& t, const Tensor& like) {
+  return t.device() == like.device() && t.scalar_type() == at::kInt && t.is_contiguous();
+}
+
+// lens, page_table, free_pages, free_count, page_size
+fdllm_page_pool page_pool(PyObject* const* a, const Tensor& ask) {
+  const Tensor &lens = tensor(a[0]), &table = tensor(a[1]), &pages = tensor(a[2]), &count = tensor(a[3]);
+  const long page = integer(a[4]);
+  plain(whole_ints(ask, lens) && whole_ints(lens, lens) && whole_ints(pages, lens) && whole_ints(count, lens) &&
+        table.device() == lens.device() && table.scalar_type() == at::kInt && table.dim() == 2 && lens.dim() == 1 &&
+        ask.dim() == 1 && pages.dim() == 1 && count.numel() == 1);
+  const int64_t B = table.size(0), most = table.size(1);
+  plain(B > 0 && B <= INT32_MAX && most <= INT32_MAX && lens.size(0) == B && ask.size(0) == B && page > 0 &&
+        page <= INT32_MAX && pages.size(0) <= INT32_MAX && (most == 0 || table.stride(1) == 1) &&
+        (B == 1 || table.stride(0) >= most));
+  on_current_device(lens);
+  fdllm_page_pool p;
+  p.page_table = static_cast<int32_t*>(table.data_ptr());
+  p.table_stride = std::max<int64_t>(table.stride(0), most);
+  p.lens = static_cast<int32_t*>(lens.data_ptr());
+  p.free_pages = static_cast<int32_t*>(pages.data_ptr());
+  p.free_count = static_cast<int32_t*>(count.data_ptr());
+  p.requests = static_cast<int>(B);
+  p.max_pages = static_cast<int>(most);
+  p.num_free = static_cast<int>(pages.size(0));
+  p.page_size = static_cast<int>(page);
+  return p;
+}
+
+PyObject* pack(std::initializer_list<Tensor*> ts) {
+  Ref out(PyTuple_New(static_cast<Py_ssize_t>(ts.size())));
+  Py_ssize_t i = 0;
+  for (Tensor* t : ts) {
+    PyObject* o = Py_None;
+    if (t->defined()) o = wrap(std::move(*t));
+    else Py_INCREF(o);
+    PyTuple_SET_ITEM(out.o, i++, o);
+  }
+  Py_INCREF(out.o);
+  return out.o;
+}
+
+// new_lens, lens, page_table, free_pages, free_count, page_size, width, rows -> PageRows' fields
+PyObject* assign(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 8);
+  const Tensor& ask = tensor(a[0]);
+  const fdllm_page_pool p = page_pool(a + 1, ask);
+  const long width = integer(a[6]), rows = integer(a[7]);
+  plain(width >= 0 && rows >= 0 && width <= INT32_MAX && rows <= INT32_MAX && (width > 0) != (rows > 0));
+  const int64_t B = p.requests;
+  Tensor slots, positions, starts, seqlens, granted, sequences, row_starts;
+  {
+    NoGil free;
+    const auto i32 = ask.options().requires_grad(false), i64 = i32.dtype(at::kLong);
+    slots = width ? at::empty({B, width}, i64) : at::empty({rows}, i64);
+    positions = at::empty(slots.sizes(), i32);
+    starts = at::empty({B}, i32);
+    seqlens = at::empty({B}, i32);
+    granted = at::empty({B}, i32);
+    if (!width) {
+      sequences = at::empty({rows}, i32);
+      row_starts = at::empty({B + 1}, i32);
+    }
+  }
+  auto ints = [](const Tensor& t) { return t.defined() ? static_cast<int32_t*>(t.data_ptr()) : nullptr; };
+  const Stream s(ask);
+  check(launch([&] { return api.assign(&p, ints(ask), static_cast<int>(width), static_cast<int>(rows),
+                   static_cast<int64_t*>(slots.data_ptr()), ints(positions), ints(sequences), ints(row_starts),
+                   ints(starts), ints(seqlens), ints(granted), s.ptr); }),
+        "fdllm_assign_pages");
+  return pack({&slots, &positions, &starts, &seqlens, &granted, &sequences, &row_starts});
+}
+
+// keep_lens, lens, page_table, free_pages, free_count, page_size -> True
+PyObject* release(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 6);
+  const Tensor& keep = tensor(a[0]);
+  const fdllm_page_pool p = page_pool(a + 1, keep);
+  const Stream s(keep);
+  check(launch([&] { return api.release(&p, static_cast<const int32_t*>(keep.data_ptr()), s.ptr); }), "fdllm_release_pages");
+  Py_RETURN_TRUE;
+}
+
+// q, k, v, positions, inv_freq, q_weight | None, k_weight | None, eps, k_cache | None, v_cache | None, slots | None,
+// interleaved, rope_scale, kv_out -> (q, k | None)
+PyObject* norm_rope(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 14);
+  const Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &pos = tensor(a[3]), &freq = tensor(a[4]);
+  const Opt qw(a[5]), kw(a[6]), kc(a[8]), vc(a[9]), slots(a[10]);
+  fdllm_norm_rope_kv_desc d = {};
+  d.eps = static_cast<float>(number(a[7]));
+  d.rope_scale = static_cast<float>(number(a[12]));
+  d.interleaved = PyObject_IsTrue(a[11]);
+  const int both = PyObject_IsTrue(a[13]);
+  if (d.interleaved < 0 || both < 0) throw PyFailed{};
+  plain(q.dim() == 4 && k.dim() == 4 && v.sizes() == k.sizes() && same(q, k) && same(q, v));
+  const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2), D = q.size(3), Hkv = k.size(2);
+  plain(k.size(0) == B && k.size(1) == S && k.size(3) == D && B * S > 0 && B <= INT32_MAX && S <= INT32_MAX &&
+        Hq <= INT32_MAX && Hkv <= INT32_MAX && D <= INT32_MAX);
+  d.dtype = dtype_code(q.scalar_type());
+  const int64_t vec = d.dtype == FDLLM_DTYPE_F32 ? 4 : 8;
+  auto rows = [&](const Tensor& t) {
+    return t.stride(3) == 1 && t.stride(0) % vec == 0 && t.stride(1) % vec == 0 && t.stride(2) % vec == 0 &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  };
+  plain(rows(q) && rows(k) && rows(v) && whole_ints(pos, q) && pos.dim() == 2 && pos.size(0) == B && pos.size(1) == S &&
+        freq.device() == q.device() && freq.scalar_type() == at::kFloat && freq.dim() == 1 && freq.is_contiguous() &&
+        2 * freq.size(0) <= D && !differentiates({&q, &k, &v, &freq, qw.t, kw.t, kc.t, vc.t}));
+  d.weight_dtype = d.dtype;
+  for (const Tensor* w : {qw.t, kw.t}) {
+    if (!w) continue;
+    plain(w->device() == q.device() && w->dim() == 1 && w->size(0) == D && w->is_contiguous() &&
+          reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0 &&
+          (w->scalar_type() == q.scalar_type() || w->scalar_type() == at::kFloat));
+    d.weight_dtype = dtype_code(w->scalar_type());
+  }
+  plain(!qw || !kw || qw->scalar_type() == kw->scalar_type());
+  plain(static_cast<bool>(kc) == static_cast<bool>(vc) && static_cast<bool>(kc) == static_cast<bool>(slots));
+  if (kc) {
+    plain(slots->device() == q.device() && slots->scalar_type() == at::kLong && slots->is_contiguous() &&
+          slots->sizes() == pos.sizes() && kc->sizes() == vc->sizes());
+    for (const Tensor* c : {kc.t, vc.t}) {
+      plain(same(q, *c) && c->dim() == 4 && c->size(2) == Hkv && c->size(3) == D && rows(*c) && c->size(1) <= INT32_MAX);
+      for (int i = 0; i < 4; ++i) plain(c->stride(i) != 0 || c->size(i) <= 1);
+    }
+    d.k_cache = kc.ptr();
+    d.k_stride_page = kc->stride(0), d.k_stride_slot = kc->stride(1), d.k_stride_ch = kc->stride(2);
+    d.v_cache = vc.ptr();
+    d.v_stride_page = vc->stride(0), d.v_stride_slot = vc->stride(1), d.v_stride_ch = vc->stride(2);
+    d.slots = static_cast<const int64_t*>(slots.ptr());
+    d.num_pages = kc->size(0);
+    d.page_size = static_cast<int>(kc->size(1));
+  }
+  on_current_device(q);
+  Tensor q_out = empty({B, S, Hq, D}, q), k_out;
+  if (both) k_out = empty({B, S, Hkv, D}, q);
+  d.q = q.data_ptr();
+  d.q_stride_b = q.stride(0), d.q_stride_s = q.stride(1), d.q_stride_h = q.stride(2);
+  d.k = k.data_ptr();
+  d.k_stride_b = k.stride(0), d.k_stride_s = k.stride(1), d.k_stride_h = k.stride(2);
+  d.v = v.data_ptr();
+  d.v_stride_b = v.stride(0), d.v_stride_s = v.stride(1), d.v_stride_h = v.stride(2);
+  d.positions = static_cast<const int32_t*>(pos.data_ptr());
+  d.inv_freq = static_cast<const float*>(freq.data_ptr());
+  d.q_weight = qw.ptr();
+  d.k_weight = kw.ptr();
+  d.q_out = q_out.data_ptr();
+  d.k_out = both ? k_out.data_ptr() : nullptr;
+  d.batch = static_cast<int>(B), d.seq_len = static_cast<int>(S), d.num_q_heads = static_cast<int>(Hq);
+  d.num_kv_heads = static_cast<int>(Hkv), d.head_dim = static_cast<int>(D);
+  d.rotary_dim = static_cast<int>(2 * freq.size(0));
+  const Stream s(q);
+  check(launch([&] { return api.norm_rope(&d, s.ptr); }), "fdllm_norm_rope_kv_write");
+  return pack({&q_out, &k_out});
+}
+
+// logits, tokens | None, top_k -> TokenLogprobs' fields
+PyObject* logprobs(PyObject* const* a, Py_ssize_t n) {
+  arity(n, 3);
+  const Tensor& x = tensor(a[0]);
+  const Opt tok(a[1]);
+  const long top = integer(a[2]);
+  const int64_t dim = x.dim();
+  plain(dim >= 1 && dim <= 3 && x.numel() > 0 && x.stride(dim - 1) == 1 && !differentiates({&x}));
+  const int dt = dtype_code(x.scalar_type());
+  const int64_t V = x.size(dim - 1), batch = dim == 3 ? x.size(0) : 1, rows = dim >= 2 ? x.size(dim - 2) : 1;
+  plain(V <= INT32_MAX && batch <= INT32_MAX && rows <= INT32_MAX && top >= 0 && top <= 32 && top <= V);
+  const auto lead = x.sizes().slice(0, dim - 1);
+  int64_t given = 0;
+  if (tok) {
+    plain(tok->device() == x.device() && tok->scalar_type() == at::kLong && tok->is_contiguous() &&
+          (tok->sizes() == lead || (tok->dim() == dim && tok->sizes().slice(0, dim - 1) == lead)));
+    given = tok->dim() == dim ? tok->size(dim - 1) : 1;
+    plain(given > 0 && given <= INT32_MAX);
+  }
+  size_t need = 0;
+  check(api.logprobs_size(static_cast<int>(V), batch * rows, dt, &need), "fdllm_token_logprobs_workspace_size");
+  on_current_device(x);
+  Tensor logp, entropy, top_logp, top_tok, parts;
+  {
+    NoGil free;
+    const auto f32 = x.options().requires_grad(false).dtype(at::kFloat);
+    if (tok) logp = at::empty(tok->sizes(), f32);
+    entropy = at::empty(lead, f32);
+    if (top) {
+      auto sizes = lead.vec();
+      sizes.push_back(top);
+      top_logp = at::empty(sizes, f32);
+      top_tok = at::empty(sizes, f32.dtype(at::kLong));
+    }
+    if (need) parts = at::empty({static_cast<int64_t>(need)}, f32.dtype(at::kByte));
+  }
+  auto floats = [](const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; };
+  const Stream s(x);
+  check(launch([&] { return api.logprobs(x.data_ptr(), dim == 3 ? x.stride(0) : 0, dim >= 2 ? x.stride(dim - 2) : 0,
+                   static_cast<int>(batch), static_cast<int>(rows), static_cast<int>(V),
+                   static_cast<const int64_t*>(tok.ptr()), static_cast<int>(given), static_cast<int>(top), floats(logp),
+                   floats(entropy), floats(top_logp), top ? static_cast<int64_t*>(top_tok.data_ptr()) : nullptr, dt,
+                   need ? parts.data_ptr() : nullptr, need, s.ptr); }),
+        "fdllm_token_logprobs");
+  return pack({&logp, &entropy, &top_logp, &top_tok});
+}
+
 // entry point addresses in Api's order, stream lookup, workspace dictionary, its get
 PyObject* init(PyObject*, PyObject* args) {
   PyObject *addr, *stream, *buffers, *get;
@@ -530,7 +745,8 @@ PyObject* init(PyObject*, PyObject* args) {
 #define FDLLM_CALL(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&call<name>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FDLLM_CALL(attn),   FDLLM_CALL(gather), FDLLM_CALL(scatter), FDLLM_CALL(add_norm),
-                         FDLLM_CALL(linear), FDLLM_CALL(linear_takes), FDLLM_CALL(qkv),    FDLLM_CALL(unmask),  {"init", init, METH_VARARGS, nullptr},
+                         FDLLM_CALL(linear), FDLLM_CALL(linear_takes), FDLLM_CALL(qkv),    FDLLM_CALL(unmask),
+                         FDLLM_CALL(assign), FDLLM_CALL(release), FDLLM_CALL(norm_rope), FDLLM_CALL(logprobs), {"init", init, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fdllm_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -124,7 +124,8 @@ class _Host:
     cannot be loaded (it is built against one torch, the kernels' library against none), every
     call takes its Python form, after one log entry."""
 
-    _CALLS = ("attn", "gather", "scatter", "add_norm", "linear", "linear_takes", "qkv", "unmask")
+    _CALLS = ("attn", "gather", "scatter", "add_norm", "linear", "linear_takes", "qkv", "unmask", "assign", "release",
+              "norm_rope", "logprobs")
 
     def __getattr__(self, name):
         if name not in self._CALLS:
@@ -966,6 +967,10 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.T
     ``lens``, ``page_table`` and ``free_count`` in place: calls on one pool run in stream order.
     """
     what = "assign_pages"
+    if new_lens.is_cuda:
+        done = _HOST.assign(new_lens, lens, page_table, free_pages, free_count, page_size, width, rows)
+        if done is not None:
+            return PageRows(*done)
     if (width > 0) == (rows > 0) or width < 0 or rows < 0:
         raise RuntimeError(f"{what}: give the padded form's width or the packed form's rows")
     p, dev = _page_pool(what, lens, page_table, free_pages, free_count, page_size, new_lens)
@@ -996,6 +1001,8 @@ def release_pages(keep_lens: torch.Tensor, lens: torch.Tensor, page_table: torch
     ends a request) and gives the pages behind back to the free list, in the reverse of
     ``assign_pages``' order: releasing a whole step leaves the pool as it was before it."""
     what = "release_pages"
+    if keep_lens.is_cuda and _HOST.release(keep_lens, lens, page_table, free_pages, free_count, page_size):
+        return
     p, dev = _page_pool(what, lens, page_table, free_pages, free_count, page_size, keep_lens)
     if keep_lens.shape != lens.shape:
         raise RuntimeError(f"{what}: keep_lens must be [B]")
@@ -1070,6 +1077,11 @@ def norm_rope_kv_write(
     with kv_out=True also the new keys [B, S, Hkv, D]. page_size is a power of two.
     """
     what = "norm_rope_kv_write"
+    if q.is_cuda:
+        done = _HOST.norm_rope(q, k, v, positions, inv_freq, q_weight, k_weight, eps, k_cache, v_cache, slots,
+                               interleaved, rope_scale, kv_out)
+        if done is not None:
+            return done if kv_out else done[0]
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         raise RuntimeError(f"{what}: q [B, S, Hq, D], k / v [B, S, Hkv, D] expected")
     B, S, Hq, D = q.shape
@@ -1166,6 +1178,10 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     is allocated by the call, so calls on several streams and captured ones are apart.
     """
     what = "token_logprobs"
+    if logits.is_cuda:
+        done = _HOST.logprobs(logits, tokens, top_k)
+        if done is not None:
+            return TokenLogprobs(*done)
     if logits.dim() < 1 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise RuntimeError(f"{what}: logits [..., V] in bf16, fp16 or fp32 expected")
     dev = _require_gpu(logits, *([tokens] if tokens is not None else []))
