@@ -10,12 +10,20 @@
 // logits near m, and the sums are trees of at most 2^-24 relative error a level.
 //
 // Alternatives without keeping a list while reading: the pass leaves the maximum of every
-// group of 2048 neighbouring logits, which the reduction makes anyway. The K first logits by
-// (larger value, lower index) lie in the K first groups by (larger maximum, lower index): a
-// logit in any other group has K logits ahead of it, those groups' maxima. Only those
-// groups are read again, and of them only what is not below the K-th maximum is ranked.
+// group of neighbouring logits that a wave loads at once (64 vectors of 16 bytes). The K-th of 64
+// maxima, each over a 64th of the groups, is a bound that K logits reach, so the K first logits
+// (larger value, then lower index) are from the bound up, and only groups whose maximum is need be
+// read again: about K of them, in which hardly more than K logits are. Where that finds too many
+// (many equal logits, sorted ones) the K-th largest value itself is found by halving the range of
+// values, then the logits above it are ranked and its first equals fill up.
 //
-// What bounds it: the one read of the logits.
+// What bounds it: many rows, the one read of the logits beside the vector units: 4 x 512 rows of 152064
+// bf16 logits (623 MB) 118 us, 5.3 TB/s, where a plain read of the memory takes 99; ten operations and an
+// exponential a logit take about 85 us of every SIMD. (x - m) log2 e is one product: the constant in two parts (a
+// multiply-add more) takes 2.4 us more and the results are no nearer to 64 bits (5.8e-8 both). Few rows, latency:
+// one fp32 row 11 us, 16 x 8 bf16 rows 17 us, of which the finish is 5: its phases are states and maxima 1.4 us,
+// bound 1.2, groups 0.3, their logits 0.9, ranks 0.7. Its code runs once a row and is loaded for it, so
+// it is kept short: with loops unrolled the finish took 9 us (K = 5) to 19 (K = 20).
 #include <math.h>
 
 #include "fdllm_common.h"
@@ -25,12 +33,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kGroup = 2048;              // neighbouring logits under one maximum: a wave's share of a step
-constexpr int kStep = kGroup * kWaves;    // logits of a workgroup's step
-constexpr int kMaxVocab = 1 << 22;
-constexpr int kMaxGroups = kMaxVocab / kGroup + 1;  // one more where a row starts off 16 bytes
+// Threads of a row's finish: 256 take 0.9 us more for 20 alternatives of one fp32 row, 1024 1.3 us
+// more (2 to 5 us where there are many rows).
+constexpr int kFinishThreads = 512;
+// Workgroups that a call aims at: 1024 take 19.0 us for 16 x 8 rows of 152064, 2048 17.2, 4096 18.1
+// (more partials, one step each); from 2048 rows on a workgroup takes whole rows.
+constexpr int kWorkgroups = 2048;
+constexpr int kStep = 2048 * kWaves;      // logits of a workgroup's step
+constexpr int kMaxVocab = 1 << 20;
 constexpr int kCandidates = 1024;
-constexpr int kMaxTop = 32;  // twice that many tokens are one wave's
+constexpr int kMaxTop = 32;
 
 struct ScoreArgs {
   const void* logits;
@@ -52,6 +64,8 @@ struct ScoreArgs {
 template <typename T>
 struct Vec {
   static constexpr int N = 8;
+  static constexpr int kGroup = 64 * N;                     // neighbouring logits under one maximum: a vector a lane
+  static constexpr int kMaxGroups = kMaxVocab / kGroup;
   __device__ __forceinline__ static void get(const u32x4& w, float* f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -66,6 +80,8 @@ struct Vec {
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
+  static constexpr int kGroup = 64 * N;
+  static constexpr int kMaxGroups = kMaxVocab / kGroup;
   __device__ __forceinline__ static void get(const u32x4& w, float* f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
@@ -83,10 +99,10 @@ struct RowVecs {
   int mis, nv;
 };
 template <typename T>
-__device__ __forceinline__ RowVecs row_of(const ScoreArgs& a, int64_t r) {
+__device__ __forceinline__ RowVecs row_of(const ScoreArgs& a, uint32_t r) {  // 32-bit division: fewer than 2^31 rows
   constexpr int N = Vec<T>::N, E = 16 / N;
-  const int64_t b = r / a.rows_per_batch;
-  const char* row = static_cast<const char*>(a.logits) + (b * a.stride_b + (r - b * a.rows_per_batch) * a.stride_r) * E;
+  const uint32_t b = r / static_cast<uint32_t>(a.rows_per_batch), i = r - b * a.rows_per_batch;
+  const char* row = static_cast<const char*>(a.logits) + (b * a.stride_b + i * a.stride_r) * E;
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / E);
   return RowVecs{reinterpret_cast<const u32x4*>(row - mis * E), row, mis, (a.V + mis + N - 1) / N};
 }
@@ -101,6 +117,13 @@ __device__ __forceinline__ void unpack(const u32x4& w, int v, const RowVecs& rv,
     for (int j = 0; j < N; ++j)
       if (j0 + j < 0 || j0 + j >= V) x[j] = -INFINITY;
   }
+}
+
+// Orders one wave's LDS accesses.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // S and A relative to the maximum m. While nothing above -inf was read they are 0, or NaN
@@ -119,6 +142,7 @@ __device__ __forceinline__ void rescale(State& x, float to) {
 }
 
 // Joins the workgroup's states; every thread returns with the row's.
+template <int NW>
 __device__ __forceinline__ State join(State x, float* s_red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float mw = wave_allreduce_max(x.m);
@@ -133,10 +157,10 @@ __device__ __forceinline__ State join(State x, float* s_red) {
   __syncthreads();
   float m = s_red[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, s_red[3 * w]);
+  for (int w = 1; w < NW; ++w) m = fmaxf(m, s_red[3 * w]);
   State r{m, 0.f, 0.f};
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < NW; ++w) {
     State y{s_red[3 * w], s_red[3 * w + 1], s_red[3 * w + 2]};
     rescale(y, m);
     r.s += y.s;
@@ -145,190 +169,248 @@ __device__ __forceinline__ State join(State x, float* s_red) {
   return r;
 }
 
-// The largest (value, lowest index) of the workgroup, to every thread.
-__device__ __forceinline__ void block_first(float& v, int& i, float* s_v, int* s_i) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float v2 = __shfl_xor(v, o, kWave);
-    const int i2 = __shfl_xor(i, o, kWave);
-    if (v2 > v || (v2 == v && i2 < i)) {
-      v = v2;
-      i = i2;
-    }
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    s_v[threadIdx.x >> 6] = v;
-    s_i[threadIdx.x >> 6] = i;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    if (s_v[w] > v || (s_v[w] == v && s_i[w] < i)) {
-      v = s_v[w];
-      i = s_i[w];
-    }
-}
-
-// f(i, rank) for every i < n of its thread: its place by (larger value, lower index).
-template <typename F>
-__device__ __forceinline__ void rank_all(const float* v, int n, F f) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const float x = v[i];
-    int rank = 0;
-    for (int h = 0; h < n; ++h) rank += v[h] > x || (v[h] == x && h < i);
-    f(i, rank);
-  }
-}
-
+struct Cand {
+  float v;
+  int i;
+};
+template <typename T, int NT>
 struct Shared {
-  float red[3 * kWaves];
-  float group[kMaxGroups];
-  float cand_v[kCandidates];
-  int cand_i[kCandidates];
-  int sel[kMaxTop];
-  float sel_v[kMaxTop];
-  int n_cand;
+  float red[3 * (NT / 64)];
+  __attribute__((aligned(16))) float lane_max[64];
+  float group[Vec<T>::kMaxGroups];
+  uint16_t sel[Vec<T>::kMaxGroups];
+  Cand cand[kCandidates];
+  float bound;
+  int n_sel, n_cand, n_above[33];
 };
 
-// A row's outputs from its state; sh.group holds its groups' maxima.
+// The given token of this thread and its logit, read ahead of the row's sums.
+struct Given {
+  bool in;
+  float x;
+};
 template <typename T>
-__device__ void finish(const ScoreArgs& a, int64_t r, const State& st, Shared& sh) {
+__device__ __forceinline__ Given given_of(const ScoreArgs& a, int64_t r, int j, const RowVecs& rv) {
+  Given g{false, 0.f};
+  if (j < a.given) {
+    const int64_t t = a.tokens[r * a.given + j];
+    g.in = t >= 0 && t < a.V;
+    if (g.in) g.x = Vec<T>::one(rv.row, t);
+  }
+  return g;
+}
+
+// Values in their order, as numbers without gaps: -inf is 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);  // -0 is 0
+  return ((b >> 31) ? ~b : b | 0x80000000u) - 0x007fffffu;
+}
+
+// A row's alternatives, by NT threads; sh.group holds its groups' maxima. The code runs once a row, so
+// its own loading counts: no loop is unrolled that need not be.
+template <typename T, int NT, typename Put>
+__device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowVecs& rv, Put put, Shared<T, NT>& sh) {
+  constexpr int N = Vec<T>::N;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int K = a.top, ng = a.n_groups;
+  // a bound that K logits reach: the K-th of 64 maxima, each over the groups that a lane takes
+  if (wave == 0) {
+    float mine = -INFINITY;
+#pragma unroll 2
+    for (int g = lane; g < ng; g += 64) mine = fmaxf(mine, sh.group[g]);
+    sh.lane_max[lane] = mine;
+    wave_sync();
+    int above = 0;
+#pragma unroll 2
+    for (int h = 0; h < 64; h += 4) {
+      const f32x4 y = *reinterpret_cast<const f32x4*>(&sh.lane_max[h]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) above += y[j] > mine;
+    }
+    const float m = -wave_allreduce_max(above < K ? -mine : -INFINITY);  // the least that fewer than K exceed
+    if (lane < 33) sh.n_above[lane] = 0;
+    if (lane == 0) {
+      sh.bound = m;
+      sh.n_sel = sh.n_cand = 0;
+    }
+  }
+  __syncthreads();
+  const float bound = sh.bound;
+  // the groups that hold a logit from the bound up
+#pragma unroll 1
+  for (int g0 = wave * 64; g0 < ng; g0 += NT) {
+    const float m = g0 + lane < ng ? sh.group[g0 + lane] : -INFINITY;
+    if (m >= bound && m > -INFINITY) sh.sel[atomicAdd(&sh.n_sel, 1)] = static_cast<uint16_t>(g0 + lane);
+  }
+  __syncthreads();
+  const int ns = sh.n_sel;
+  // f(a vector of those groups, its number), the next one in flight
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    int v = 0;
+    u32x4 next;
+    auto fetch = [&](int i) __attribute__((always_inline)) {
+      if (i < ns) {
+        v = sh.sel[i] * 64 + lane;
+        if (v < rv.nv) next = rv.v[v];
+      }
+    };
+    fetch(wave);
+#pragma unroll 1
+    for (int i = wave; i < ns; i += NT / 64) {
+      const u32x4 w = next;
+      const int at = v;
+      fetch(i + NT / 64);
+      if (at < rv.nv) f(w, at);
+    }
+  };
+  // those from `than` up (without its equals, if strict) into the list
+  auto collect = [&](float than, bool strict) __attribute__((always_inline)) {
+    each([&](const u32x4& w, int v) __attribute__((always_inline)) {
+      float x[N];
+      unpack<T>(w, v, rv, a.V, x);
+      uint32_t in = 0;
+#pragma unroll
+      for (int j = 0; j < N; ++j) in |= ((x[j] > than || (x[j] == than && !strict)) && x[j] > -INFINITY ? 1u : 0u) << j;
+      if (in == 0) return;
+      int c = atomicAdd(&sh.n_cand, __builtin_popcount(in));
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if ((in >> j & 1) && c < kCandidates) sh.cand[c++] = Cand{x[j], N * v + j - rv.mis};
+      }
+    });
+    __syncthreads();
+  };
+  collect(bound, false);
+  int n = sh.n_cand;
+  float rest = -INFINITY;  // what is left to take is equal to this
+  if (__builtin_expect(n > kCandidates, 0)) {
+    // Too many (equal logits, sorted ones): the K-th largest value itself, by halving the range of
+    // values that it can have; at most K - 1 logits are above it
+    uint32_t lo = order_of(bound), hi = 0xff800000u;  // more than K - 1 logits reach lo, no finite one hi
+    int round = 0;
+#pragma unroll 1
+    for (uint32_t mid = lo + 1; lo + 1 < hi; mid = lo + (hi - lo) / 2, ++round) {
+      int c = 0;
+      each([&](const u32x4& w, int v) __attribute__((always_inline)) {
+        float x[N];
+        unpack<T>(w, v, rv, a.V, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) c += order_of(x[j]) >= mid;
+      });
+      c = static_cast<int>(wave_allreduce_sum(static_cast<float>(c)));  // at most 2^20: exact
+      if (lane == 0) atomicAdd(&sh.n_above[round], c);
+      __syncthreads();
+      if (sh.n_above[round] >= K) lo = mid;
+      else hi = mid;
+    }
+    const uint32_t b = lo + 0x007fffffu;
+    rest = __uint_as_float((b >> 31) ? b & 0x7fffffffu : ~b);
+    if (tid == 0) sh.n_cand = 0;
+    __syncthreads();
+    collect(rest, true);
+    n = sh.n_cand;
+  }
+  // eight threads rank one: a loop over them all by itself is a chain of LDS latencies
+#pragma unroll 1
+  for (int c = tid >> 3; c < n; c += NT / 8) {
+    const Cand mine = sh.cand[c];
+    float rank = 0.f;
+#pragma unroll 2
+    for (int h = tid & 7; h < n; h += 8) {
+      const Cand o = sh.cand[h];
+      rank += o.v > mine.v || (o.v == mine.v && o.i < mine.i) ? 1.f : 0.f;
+    }
+    rank += dpp_f32<0xB1>(rank);
+    rank += dpp_f32<0x4E>(rank);
+    rank += dpp_f32<0x141>(rank);
+    if ((tid & 7) == 0 && rank < K) put(static_cast<int>(rank), mine.v, mine.i);
+  }
+  // fewer than K: of those equal to `rest`, the first ones
+  if (__builtin_expect(n < K, 0) && wave == 0) {
+#pragma unroll 1
+    for (int i0 = 0; i0 < a.V && n < K; i0 += 64) {
+      const bool in = i0 + lane < a.V && Vec<T>::one(rv.row, i0 + lane) == rest;
+      const uint64_t all = __builtin_amdgcn_ballot_w64(in);
+      const int rank = n + __builtin_popcountll(all & ((1ull << lane) - 1));
+      if (in && rank < K) put(rank, rest, i0 + lane);
+      n += __builtin_popcountll(all);
+    }
+  }
+}
+
+// A row's outputs from its state, by NT threads; g: the thread's given token.
+template <typename T, int NT>
+__device__ __forceinline__ void finish(const ScoreArgs& a, int64_t r, const RowVecs& rv, const State& st, Given g,
+                                       Shared<T, NT>& sh) {
   const int tid = threadIdx.x;
-  const RowVecs rv = row_of<T>(a, r);
   // a NaN or +inf logit makes the sum NaN, a row without a finite one leaves it 0
   const bool good = st.s > 0.f;
   const float lse = logf(st.s);
   const float nan = __builtin_nanf("");
   if (tid == 0) a.entropy[r] = good ? lse - st.a / st.s : nan;
-  for (int j = tid; j < a.given; j += kThreads) {
-    const int64_t t = a.tokens[r * a.given + j];
-    a.logprobs[r * a.given + j] = good && t >= 0 && t < a.V ? Vec<T>::one(rv.row, t) - st.m - lse : nan;
+#pragma unroll 1
+  for (int j = tid; j < a.given; j += NT) {
+    a.logprobs[r * a.given + j] = good && g.in ? g.x - st.m - lse : nan;
+    g = given_of<T>(a, r, j + NT, rv);
   }
   const int K = a.top;
-  if (K == 0) return;
-  if (!good) {  // uniform
-    for (int k = tid; k < K; k += kThreads) {
-      a.top_tokens[r * K + k] = -1;
-      a.top_logprobs[r * K + k] = nan;
-    }
-    return;
+  if (good && K > 0) {  // uniform
+    alternatives<T, NT>(a, rv, [&](int k, float v, int i) __attribute__((always_inline)) {
+      a.top_tokens[r * K + k] = i;
+      a.top_logprobs[r * K + k] = v - st.m - lse;
+    }, sh);
+  } else if (tid < K) {
+    a.top_tokens[r * K + tid] = -1;
+    a.top_logprobs[r * K + tid] = nan;
   }
-  auto put = [&](int k, float v, int i) __attribute__((always_inline)) {
-    a.top_tokens[r * K + k] = i;
-    a.top_logprobs[r * K + k] = v - st.m - lse;
-  };
-  // the K first groups
-  const int ng = a.n_groups;
-  rank_all(sh.group, ng, [&](int g, int rank) __attribute__((always_inline)) {
-    if (rank < K) {
-      sh.sel[rank] = g;
-      sh.sel_v[rank] = sh.group[g];
-    }
-  });
-  if (tid == 0) sh.n_cand = 0;
-  __syncthreads();
-  const int ns = min(ng, K);
-  // every logit of those groups: f(value, index)
-  constexpr int N = Vec<T>::N, GV = kGroup / N;
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    for (int q = tid; q < ns * GV; q += kThreads) {
-      const int v = sh.sel[q / GV] * GV + q % GV;
-      if (v >= rv.nv) continue;
-      float x[N];
-      unpack<T>(rv.v[v], v, rv, a.V, x);
+}
+
+// The maximum over the lanes of each of the U values m[u], the u-th group's: where it is, value u of the
+// wave's U / 4 to a lane. Lanes trade halves of their values for halves of the others', so that two and
+// a few exchanges serve all.
+template <int U>
+__device__ __forceinline__ void group_maxima(float* m, int lane) {
+  const bool up32 = (lane & 32) != 0, up16 = (lane & 16) != 0;
 #pragma unroll
-      for (int j = 0; j < N; ++j) f(x[j], N * v + j - rv.mis);  // -inf outside of the row
-    }
-  };
-  float least = ng < K ? -INFINITY : sh.sel_v[K - 1];
-  int n = 0;
-  // With fewer groups than K, or too many logits from their K-th maximum up (sorted ones), the
-  // K-th of the threads' own maxima is the bound: K threads have a logit that reaches it.
-  for (int round = ng < K ? 1 : 0; round < 2; ++round) {
-    if (round == 1) {
-      float m = -INFINITY;
-      each([&](float x, int) __attribute__((always_inline)) { m = fmaxf(m, x); });
-      sh.cand_v[tid] = m;
-      __syncthreads();
-      rank_all(sh.cand_v, kThreads, [&](int t, int rank) __attribute__((always_inline)) {
-        if (rank == K - 1) sh.sel_v[0] = sh.cand_v[t];
-      });
-      if (tid == 0) sh.n_cand = 0;
-      __syncthreads();
-      least = sh.sel_v[0];
-    }
-    each([&](float x, int at) __attribute__((always_inline)) {
-      if (x >= least && x > -INFINITY) {
-        const int c = atomicAdd(&sh.n_cand, 1);
-        if (c < kCandidates) {
-          sh.cand_v[c] = x;
-          sh.cand_i[c] = at;
-        }
-      }
-    });
-    __syncthreads();
-    n = sh.n_cand;
-    __syncthreads();  // read before another round clears it
-    if (n <= kCandidates) break;
+  for (int u = 0; u < U / 2; ++u) {
+    const float give = up32 ? m[u] : m[u + U / 2], own = up32 ? m[u + U / 2] : m[u];
+    m[u] = fmaxf(own, __shfl_xor(give, 32, kWave));
   }
-  if (n <= kCandidates) {
-    for (int c = tid; c < n; c += kThreads) {
-      const float v = sh.cand_v[c];
-      const int i = sh.cand_i[c];
-      int rank = 0;
-      for (int h = 0; h < n; ++h) rank += sh.cand_v[h] > v || (sh.cand_v[h] == v && sh.cand_i[h] < i);
-      if (rank < K) put(rank, v, i);
-    }
-    // fewer than K above -inf: the excluded tokens of lowest index, which are among the first 2 K
-    if (n < K && tid < 64) {
-      const bool out = tid < a.V && Vec<T>::one(rv.row, tid) == -INFINITY;
-      const uint64_t all = __builtin_amdgcn_ballot_w64(out);
-      const int rank = n + __builtin_popcountll(all & ((1ull << tid) - 1));
-      if (out && rank < K) put(rank, -INFINITY, tid);
-    }
-    return;
-  }
-  // many equal logits: one at a time
-  float last_v = INFINITY;
-  int last_i = -1;
-  for (int k = 0; k < K; ++k) {
-    float bv = -INFINITY;
-    int bi = 0x7fffffff;
-    each([&](float x, int at) __attribute__((always_inline)) {
-      const bool after = x < last_v || (x == last_v && at > last_i);
-      if (after && (x > bv || (x == bv && at < bi))) {
-        bv = x;
-        bi = at;
-      }
-    });
-    block_first(bv, bi, sh.red, reinterpret_cast<int*>(sh.red + kWaves));
-    if (tid == 0) put(k, bv, bi);
-    last_v = bv;
-    last_i = bi;
+#pragma unroll
+  for (int u = 0; u < U / 4; ++u) {
+    const float give = up16 ? m[u] : m[u + U / 4], own = up16 ? m[u + U / 4] : m[u];
+    m[u] = fmaxf(own, __shfl_xor(give, 16, kWave));
+    m[u] = fmaxf(m[u], dpp_f32<0xB1>(m[u]));
+    m[u] = fmaxf(m[u], dpp_f32<0x4E>(m[u]));
+    m[u] = fmaxf(m[u], dpp_f32<0x141>(m[u]));
+    m[u] = fmaxf(m[u], dpp_f32<0x140>(m[u]));
   }
 }
 
 // One workgroup per row, or per `steps` steps of a row that several share.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
-  constexpr int N = Vec<T>::N, GV = kGroup / N, U = GV / 64;  // vectors of a group, of a lane in it
-  __shared__ Shared sh;
-  const int64_t r = blockIdx.x / a.splits;
-  const int split = static_cast<int>(blockIdx.x - r * a.splits);
+__global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
+  constexpr int N = Vec<T>::N, U = kStep / kWaves / Vec<T>::kGroup;  // a lane's vectors in a step
+  __shared__ Shared<T, kThreads> sh;
+  const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.splits);
+  const int split = static_cast<int>(blockIdx.x - row * a.splits);
+  const int64_t r = row;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const RowVecs rv = row_of<T>(a, r);
+  const RowVecs rv = row_of<T>(a, row);
   float* groups = a.parts + a.rows * a.splits * 4 + r * a.n_groups;  // splits > 1
   State st{-INFINITY, 0.f, 0.f};
+  Given given{false, 0.f};
+  if (a.splits == 1) given = given_of<T>(a, r, threadIdx.x, rv);
+#pragma unroll 1
   for (int k = 0; k < a.steps; ++k) {
-    const int g = (split * a.steps + k) * kWaves + wave;
-    const int v0 = g * GV + lane;
+    const int g = ((split * a.steps + k) * kWaves + wave) * U;
+    const int v0 = g * 64 + lane;
     if (g >= a.n_groups) break;  // uniform over the wave
     u32x4 w[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (v0 + 64 * u < rv.nv) w[u] = __builtin_nontemporal_load(rv.v + v0 + 64 * u);
-    float x[U][N];
+    float x[U][N], mu[U];
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -338,8 +420,10 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
 #pragma unroll
         for (int j = 0; j < N; ++j) x[u][j] = -INFINITY;
       }
+      mu[u] = x[u][0];
 #pragma unroll
-      for (int j = 0; j < N; ++j) m = fmaxf(m, x[u][j]);
+      for (int j = 1; j < N; ++j) mu[u] = fmaxf(mu[u], x[u][j]);
+      m = fmaxf(m, mu[u]);
     }
     if (m > st.m) rescale(st, m);
     const float ref = st.m == -INFINITY ? 0.f : st.m;
@@ -348,62 +432,80 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float t = x[u][j] - ref;
-        // exp2 of the product with log2 e in two parts: with one, the constant's rounding
-        // biases every term the same way
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(t, 1.44269502f, t * 1.92596299e-8f));
+        const float e = __builtin_amdgcn_exp2f(t * 1.44269504f);
         st.s += e;
         st.a = __builtin_fmaf(e, fmaxf(t, -1e30f), st.a);  // a banned token's 0 times -inf counts as 0
       }
     if (a.top > 0) {
-      m = wave_allreduce_max(m);
-      if (lane == 0) {
-        if (a.splits > 1) groups[g] = m;
-        else sh.group[g] = m;
+      group_maxima<U>(mu, lane);
+      const int u0 = (lane >> 5) * (U / 2) + ((lane >> 4) & 1) * (U / 4);
+      if ((lane & 15) == 0) {
+#pragma unroll
+        for (int u = 0; u < U / 4; ++u)
+          if (g + u0 + u < a.n_groups) {
+            if (a.splits > 1) groups[g + u0 + u] = mu[u];
+            else sh.group[g + u0 + u] = mu[u];
+          }
       }
     }
   }
-  st = join(st, sh.red);  // a barrier: the group maxima are in LDS after it
+  st = join<kWaves>(st, sh.red);  // a barrier: the group maxima are in LDS after it
   if (a.splits == 1) {
-    finish<T>(a, r, st, sh);
+    finish<T, kThreads>(a, r, rv, st, given, sh);
   } else if (threadIdx.x == 0) {
     reinterpret_cast<float4*>(a.parts)[blockIdx.x] = make_float4(st.m, st.s, st.a, 0.f);
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void score_finish_kernel(const ScoreArgs a) {
-  __shared__ Shared sh;
+__global__ __launch_bounds__(kFinishThreads) void score_finish_kernel(const ScoreArgs a) {
+  __shared__ Shared<T, kFinishThreads> sh;
   const int64_t r = blockIdx.x;
+  const RowVecs rv = row_of<T>(a, blockIdx.x);
+  const int tid = threadIdx.x;
+  // what is read of the row: the workgroups' states by the first wave, the groups' maxima by all
   const float4* parts = reinterpret_cast<const float4*>(a.parts) + r * a.splits;
-  State st{-INFINITY, 0.f, 0.f};
-  for (int s = threadIdx.x; s < a.splits; s += kThreads) {
-    const float4 p = parts[s];
-    State y{p.x, p.y, p.z};
-    const float m = fmaxf(st.m, y.m);
-    rescale(st, m);
-    rescale(y, m);
-    st.s += y.s;
-    st.a += y.a;
-  }
+  const float* groups = a.parts + a.rows * a.splits * 4 + r * a.n_groups;
+  float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  if (tid < a.splits) p = parts[tid];
   if (a.top > 0) {
-    const float* groups = a.parts + a.rows * a.splits * 4 + r * a.n_groups;
-    for (int g = threadIdx.x; g < a.n_groups; g += kThreads) sh.group[g] = groups[g];
+#pragma unroll 1
+    for (int g = tid; g < a.n_groups; g += kFinishThreads) sh.group[g] = groups[g];
   }
-  st = join(st, sh.red);
-  finish<T>(a, r, st, sh);
+  const Given given = given_of<T>(a, r, tid, rv);
+  if (tid < 64) {
+    State st{p.x, p.y, p.z};
+#pragma unroll 1
+    for (int s = tid + 64; s < a.splits; s += 64) {
+      const float4 q = parts[s];
+      State y{q.x, q.y, q.z};
+      const float m = fmaxf(st.m, y.m);
+      rescale(st, m);
+      rescale(y, m);
+      st.s += y.s;
+      st.a += y.a;
+    }
+    rescale(st, wave_allreduce_max(st.m));
+    sh.red[0] = st.m;
+    sh.red[1] = wave_allreduce_sum(st.s);
+    sh.red[2] = wave_allreduce_sum(st.a);
+  }
+  __syncthreads();
+  finish<T, kFinishThreads>(a, r, rv, State{sh.red[0], sh.red[1], sh.red[2]}, given, sh);
 }
 
 struct Cut {
   int n_groups, steps, splits;
   size_t bytes;
 };
-// Rows are shared by workgroups until there are about eight for every compute unit.
+// Rows are shared by workgroups until there are kWorkgroups of them.
 Cut cut(int vocab, int64_t rows, int dtype) {
   Cut c;
   const int slack = dtype == FDLLM_DTYPE_F32 ? 3 : 7;  // a row may start inside a vector
-  c.n_groups = (vocab + slack + kGroup - 1) / kGroup;
-  const int64_t all = (c.n_groups + kWaves - 1) / kWaves;
-  const int64_t want = rows < 2048 ? 2048 / rows : 1;
+  const int group = dtype == FDLLM_DTYPE_F32 ? Vec<float>::kGroup : Vec<bf16_t>::kGroup;
+  c.n_groups = (vocab + slack + group - 1) / group;
+  const int64_t all = (static_cast<int64_t>(c.n_groups) * group + kStep - 1) / kStep;
+  const int64_t want = rows < kWorkgroups ? kWorkgroups / rows : 1;
   const int64_t splits = want < all ? want : all;
   c.steps = static_cast<int>((all + splits - 1) / splits);
   c.splits = static_cast<int>((all + c.steps - 1) / c.steps);
@@ -414,7 +516,7 @@ Cut cut(int vocab, int64_t rows, int dtype) {
 template <typename T>
 void launch(const ScoreArgs& a, hipStream_t s) {
   score_kernel<T><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(kThreads), 0, s>>>(a);
-  if (a.splits > 1) score_finish_kernel<T><<<dim3(static_cast<unsigned>(a.rows)), dim3(kThreads), 0, s>>>(a);
+  if (a.splits > 1) score_finish_kernel<T><<<dim3(static_cast<unsigned>(a.rows)), dim3(kFinishThreads), 0, s>>>(a);
 }
 
 int check_sizes(const char* what, int vocab, int64_t rows, int dtype) {

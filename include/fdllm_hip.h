@@ -601,7 +601,7 @@ int fdllm_norm_rope_kv_write(const fdllm_norm_rope_kv_desc* desc, void* stream);
  *
  * `workspace` (fdllm_token_logprobs_workspace_size bytes, 0 for many rows; 16-byte aligned)
  * needs no initialisation; calls that may overlap in time need separate ones. One kernel, or two
- * where workgroups share a row. vocab is at most 2^22 - 8.
+ * where workgroups share a row. vocab is at most 2^20 - 8.
  *
  * No counterpart in the reference, whose sampling takes the probability of the greedy token
  * (modeling.py:2263-2270); for scoring given texts.
