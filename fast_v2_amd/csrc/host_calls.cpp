@@ -173,6 +173,32 @@ Tensor empty(at::IntArrayRef sizes, const Tensor& like) {
   return at::empty(sizes, like.options().requires_grad(false));
 }
 
+// Several outputs in one allocation (an allocation takes a microsecond, these views a tenth), each
+// from a multiple of 256 bytes on.
+class Carve {
+ public:
+  int64_t add(int64_t n, size_t size) {
+    const int64_t at = bytes_;
+    bytes_ += (n * static_cast<int64_t>(size) + 255) / 256 * 256;
+    return at;
+  }
+  void allocate(const Tensor& like) {
+    NoGil free;
+    base_ = at::empty({std::max<int64_t>(bytes_, 1)}, like.options().requires_grad(false).dtype(at::kByte));
+  }
+  Tensor view(int64_t at, at::IntArrayRef sizes, at::ScalarType type) const {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(),
+                                                        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(type)));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+  }
+
+ private:
+  int64_t bytes_ = 0;
+  Tensor base_;
+};
+
 template <typename F>
 int launch(F f) {
   NoGil free;
@@ -564,19 +590,20 @@ PyObject* assign(PyObject* const* a, Py_ssize_t n) {
   const long width = integer(a[6]), rows = integer(a[7]);
   plain(width >= 0 && rows >= 0 && width <= INT32_MAX && rows <= INT32_MAX && (width > 0) != (rows > 0));
   const int64_t B = p.requests;
-  Tensor slots, positions, starts, seqlens, granted, sequences, row_starts;
-  {
-    NoGil free;
-    const auto i32 = ask.options().requires_grad(false), i64 = i32.dtype(at::kLong);
-    slots = width ? at::empty({B, width}, i64) : at::empty({rows}, i64);
-    positions = at::empty(slots.sizes(), i32);
-    starts = at::empty({B}, i32);
-    seqlens = at::empty({B}, i32);
-    granted = at::empty({B}, i32);
-    if (!width) {
-      sequences = at::empty({rows}, i32);
-      row_starts = at::empty({B + 1}, i32);
-    }
+  const int64_t n_rows = width ? B * width : rows;
+  plain(n_rows <= INT32_MAX);
+  Carve all;
+  const int64_t at[] = {all.add(n_rows, 8), all.add(n_rows, 4), all.add(B, 4), all.add(B, 4), all.add(B, 4),
+                        all.add(width ? 0 : rows, 4), all.add(width ? 0 : B + 1, 4)};
+  all.allocate(ask);
+  const int64_t grid[] = {B, width};
+  const at::IntArrayRef shape = width ? at::IntArrayRef(grid) : at::IntArrayRef(rows);
+  Tensor slots = all.view(at[0], shape, at::kLong), positions = all.view(at[1], shape, at::kInt),
+         starts = all.view(at[2], {B}, at::kInt), seqlens = all.view(at[3], {B}, at::kInt),
+         granted = all.view(at[4], {B}, at::kInt), sequences, row_starts;
+  if (!width) {
+    sequences = all.view(at[5], {rows}, at::kInt);
+    row_starts = all.view(at[6], {B + 1}, at::kInt);
   }
   auto ints = [](const Tensor& t) { return t.defined() ? static_cast<int32_t*>(t.data_ptr()) : nullptr; };
   const Stream s(ask);
@@ -692,19 +719,21 @@ PyObject* logprobs(PyObject* const* a, Py_ssize_t n) {
   size_t need = 0;
   check(api.logprobs_size(static_cast<int>(V), batch * rows, dt, &need), "fdllm_token_logprobs_workspace_size");
   on_current_device(x);
-  Tensor logp, entropy, top_logp, top_tok, parts;
-  {
+  const int64_t total = batch * rows;
+  Carve all;
+  const int64_t at[] = {all.add(tok ? tok->numel() : 0, 4), all.add(total, 4), all.add(total * top, 4), all.add(total * top, 8)};
+  all.allocate(x);
+  Tensor logp, entropy = all.view(at[1], lead, at::kFloat), top_logp, top_tok, parts;
+  if (tok) logp = all.view(at[0], tok->sizes(), at::kFloat);
+  if (top) {
+    auto sizes = lead.vec();
+    sizes.push_back(top);
+    top_logp = all.view(at[2], sizes, at::kFloat);
+    top_tok = all.view(at[3], sizes, at::kLong);
+  }
+  if (need) {
     NoGil free;
-    const auto f32 = x.options().requires_grad(false).dtype(at::kFloat);
-    if (tok) logp = at::empty(tok->sizes(), f32);
-    entropy = at::empty(lead, f32);
-    if (top) {
-      auto sizes = lead.vec();
-      sizes.push_back(top);
-      top_logp = at::empty(sizes, f32);
-      top_tok = at::empty(sizes, f32.dtype(at::kLong));
-    }
-    if (need) parts = at::empty({static_cast<int64_t>(need)}, f32.dtype(at::kByte));
+    parts = at::empty({static_cast<int64_t>(need)}, x.options().requires_grad(false).dtype(at::kByte));
   }
   auto floats = [](const Tensor& t) { return t.defined() ? static_cast<float*>(t.data_ptr()) : nullptr; };
   const Stream s(x);

@@ -14,7 +14,8 @@
 // of many requests.
 //
 // What bounds it: latency. The bytes of the largest call take 0.2 us; the calls are chains
-// of dependent memory round trips (lengths, free list or table, stores).
+// of dependent memory round trips (arguments, lengths, free list or table, stores) and the scans' barriers:
+// 16 x 8 rows 3.5 us and 2.4 us to release them, 2048 x 32 rows (4096 pages) 8.5 + 2.6 and 4.7.
 #include "fdllm_common.h"
 
 namespace fdllm {
@@ -22,6 +23,9 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxRequests = 8192;
+// Rows up to which the plan's workgroup makes them too. us, one kernel / two (assign and release): 16 x 8
+// rows 5.9 / 7.3, 256 x 16 8.4 / 9.3, 256 x 32 11.0 / 10.1, 1024 x 16 15.2 / 10.7, 2048 x 32 42 / 15.3.
+constexpr int kOneKernelRows = 4096;
 
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
@@ -48,15 +52,21 @@ __device__ __forceinline__ Scan block_scan(uint32_t x, uint32_t* s_wave) {
   return r;
 }
 
-// First b < n with upto[b] > i (n if there is none).
-__device__ __forceinline__ int first_above(const uint32_t* upto, int n, uint32_t i) {
-  int lo = 0, hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (upto[mid] > i) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
+// First b with upto[b] > i, of N (a power of two) entries; N where there is none. Without branches, so
+// that several searches run side by side.
+template <int N>
+__device__ __forceinline__ int first_above(const uint32_t* upto, uint32_t i) {
+  int at = 0;
+#pragma unroll
+  for (int s = N / 2; s >= 1; s /= 2) at += upto[at + s - 1] <= i ? s : 0;
+  return at + (upto[at] <= i ? 1 : 0);
+}
+
+// Pages of a thread at a time: many requests need them (2048 x 32 rows 17.7 us with one, 15.3 with four), few
+// are quicker in little code (16 x 8 rows 6.0 and 6.8).
+template <int ITEMS>
+constexpr int side() {
+  return ITEMS == 1 ? 1 : 4;
 }
 
 struct AssignArgs {
@@ -72,43 +82,52 @@ struct AssignArgs {
   int32_t* granted;
 };
 
-// A row's slot and position, given its request's numbers.
-__device__ __forceinline__ void put_row(const AssignArgs& a, int64_t r, int b, bool live, int64_t pos, int64_t slot) {
+// Row r: the request's t-th asked token (b < 0: none), at position pos.
+__device__ __forceinline__ void put_row(const AssignArgs& a, int r, int b, int64_t pos, int64_t slot) {
   a.slots[r] = slot;
-  a.positions[r] = live ? static_cast<int32_t>(pos) : 0;
-  if (a.sequences) a.sequences[r] = live ? b : -1;
+  a.positions[r] = static_cast<int32_t>(pos);
+  if (a.sequences) a.sequences[r] = b;
 }
 
-// The requests' part: one workgroup, ITEMS consecutive requests per thread.
-template <int ITEMS>
-__global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignArgs a) {
+// The requests' part, and in the form of one kernel (ROWS) the rows': one workgroup, ITEMS
+// consecutive requests per thread.
+template <int ITEMS, bool ROWS>
+__global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignArgs a, int n_rows) {
   __shared__ uint32_t s_wave[2][kPlanThreads / 64];
   __shared__ uint32_t s_upto[kPlanThreads * ITEMS];  // running sum of the needs
   __shared__ int32_t s_at[kPlanThreads * ITEMS];     // table column of page i: s_at + i
+  __shared__ uint32_t s_end[ROWS ? kPlanThreads * ITEMS : 1];  // running sum of the asked tokens
+  __shared__ uint32_t s_len[ROWS ? kPlanThreads * ITEMS : 1];  // length, the top bit: granted
+  __shared__ uint32_t s_new[ROWS ? kPlanThreads * ITEMS : 1];
   __shared__ uint32_t s_taken;
+  constexpr int kSide = side<ITEMS>();
   const fdllm_page_pool& p = a.pool;
   const int tid = threadIdx.x;
-  const uint32_t avail = static_cast<uint32_t>(min(max(*p.free_count, 0), p.num_free));
   const uint32_t mask = (1u << a.shift) - 1;
   if (tid == 0) s_taken = 0;
+  const int count = *p.free_count;
   uint32_t n[ITEMS], len[ITEMS], need[ITEMS], have[ITEMS];
+  int32_t old[ITEMS];
   bool asks[ITEMS];
   uint32_t sum_n = 0, sum_need = 0;
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int b = tid * ITEMS + k;
     n[k] = b < p.requests ? max(a.new_lens[b], 0) : 0;
-    len[k] = b < p.requests ? max(p.lens[b], 0) : 0;
+    old[k] = b < p.requests ? p.lens[b] : 0;
+    len[k] = max(old[k], 0);
     sum_n = add_sat(sum_n, n[k]);
   }
   // rows first (their sum does not depend on what is granted), then the needs of those that fit
-  uint32_t at = block_scan(sum_n, s_wave[0]).before;
+  uint32_t at = a.width > 0 ? 0 : block_scan(sum_n, s_wave[0]).before;
+  const uint32_t avail = static_cast<uint32_t>(min(max(count, 0), p.num_free));
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int b = tid * ITEMS + k;
     if (a.row_starts && b < p.requests) a.row_starts[b] = static_cast<int32_t>(min(at, 0x7fffffffu));
     at = add_sat(at, n[k]);
     if (a.row_starts && b == p.requests - 1) a.row_starts[p.requests] = static_cast<int32_t>(min(at, 0x7fffffffu));
+    if (ROWS) s_end[b] = at;
     // lengths are below 2^31, so their sum fits 32 unsigned bits
     const uint32_t total = (len[k] + n[k] + mask) >> a.shift;
     have[k] = (len[k] + mask) >> a.shift;
@@ -127,51 +146,97 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
     s_upto[b] = c;
     const bool ok = asks[k] && (need[k] == 0 || c <= avail);
     if (ok) taken = max(taken, need[k] ? c : 0);
+    const uint32_t got = ok ? n[k] : 0;
+    if (ROWS) {
+      s_len[b] = len[k] | (ok ? 0x80000000u : 0);
+      s_new[b] = n[k];
+    }
     if (b < p.requests) {
-      const int32_t old = p.lens[b];
-      const uint32_t got = ok ? n[k] : 0;
       a.starts[b] = static_cast<int32_t>(len[k]);
       a.seqlens[b] = static_cast<int32_t>(len[k] + got);
       a.granted[b] = static_cast<int32_t>(got);
-      if (ok) p.lens[b] = static_cast<int32_t>(len[k] + got);
-      else if (old < 0) p.lens[b] = 0;
+      if (got != 0 || old[k] < 0) p.lens[b] = static_cast<int32_t>(len[k] + got);
     }
   }
   if (taken) atomicMax(&s_taken, taken);
   __syncthreads();
   taken = s_taken;
-  for (uint32_t i = tid; i < taken; i += kPlanThreads) {
-    const int b = first_above(s_upto, p.requests, i);
-    p.page_table[b * p.table_stride + static_cast<int32_t>(s_at[b] + i)] = p.free_pages[avail - 1 - i];
-  }
   if (tid == 0) *p.free_count = static_cast<int32_t>(avail - taken);
+  for (uint32_t i0 = tid; i0 < taken; i0 += kSide * kPlanThreads) {
+    int b[kSide], page[kSide];
+#pragma unroll
+    for (int k = 0; k < kSide; ++k) {
+      const uint32_t i = min(i0 + k * kPlanThreads, taken - 1);  // the last one may be written twice
+      b[k] = first_above<kPlanThreads * ITEMS>(s_upto, i);
+      page[k] = p.free_pages[avail - 1 - i];
+    }
+#pragma unroll
+    for (int k = 0; k < kSide; ++k) {
+      const uint32_t i = min(i0 + k * kPlanThreads, taken - 1);
+      p.page_table[b[k] * p.table_stride + static_cast<int32_t>(s_at[b[k]] + i)] = page[k];
+    }
+  }
+  if constexpr (ROWS) {
+#pragma unroll 1
+    for (int r = tid; r < n_rows; r += kPlanThreads) {
+      int b, t;
+      if (a.width > 0) {
+        b = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(a.width));
+        t = r - b * a.width;
+        if (static_cast<uint32_t>(t) >= s_new[b]) b = -1;
+      } else {
+        b = first_above<kPlanThreads * ITEMS>(s_end, static_cast<uint32_t>(r));
+        t = b < p.requests ? r - static_cast<int>(s_end[b] - s_new[b]) : 0;  // an end past r and a begin at most r: no saturation
+        if (b >= p.requests) b = -1;
+      }
+      int64_t pos = 0, slot = -1;
+      if (b >= 0) {
+        const uint32_t l = s_len[b];
+        pos = static_cast<int64_t>(l & 0x7fffffffu) + t;
+        if (l >> 31) {
+          // a page in hand from the table, a new one from the free list: this kernel's stores need not be read back
+          const uint32_t j = static_cast<uint32_t>(pos >> a.shift);
+          const int32_t page = j < (((l & 0x7fffffffu) + mask) >> a.shift) ? p.page_table[b * p.table_stride + j]
+                                                                          : p.free_pages[avail - 1 - (j - s_at[b])];
+          slot = (static_cast<int64_t>(page) << a.shift) + (pos & mask);
+        }
+      }
+      put_row(a, r, b, pos, slot);
+    }
+  }
 }
 
-// The rows' part, after the plan.
-__global__ __launch_bounds__(256) void assign_rows_kernel(const AssignArgs a, int64_t n_rows) {
+// The rows' part by itself, after the plan: their begins in LDS where they have to be searched.
+constexpr int kRowsPerWg = 256;  // with 1024 rows the searches of 16384 take 7.4 us in place of 4.2
+template <int N>  // at least as many requests
+__global__ __launch_bounds__(kRowsPerWg) void assign_rows_kernel(const AssignArgs a, int n_rows) {
+  __shared__ uint32_t s_end[N];
   const fdllm_page_pool& p = a.pool;
-  for (int64_t r = blockIdx.x * 256ll + threadIdx.x; r < n_rows; r += gridDim.x * 256ll) {
-    int b, t;
-    bool live;
-    if (a.width > 0) {
-      b = static_cast<int>(r / a.width);
-      t = static_cast<int>(r - static_cast<int64_t>(b) * a.width);
-      live = t < a.new_lens[b];
-    } else {
-      // the last request that begins at or before r and is not empty: the first whose end is above r
-      b = first_above(reinterpret_cast<const uint32_t*>(a.row_starts + 1), p.requests, static_cast<uint32_t>(r));
-      live = b < p.requests;
-      t = live ? static_cast<int>(r) - a.row_starts[b] : 0;
-    }
-    int64_t pos = 0, slot = -1;
-    if (live) {
-      pos = static_cast<int64_t>(a.starts[b]) + t;
-      if (a.granted[b] > 0)
-        slot = (static_cast<int64_t>(p.page_table[b * p.table_stride + (pos >> a.shift)]) << a.shift) +
-               (pos & ((1 << a.shift) - 1));
-    }
-    put_row(a, r, b, live, pos, slot);
+  if (a.width == 0) {
+    for (int b = threadIdx.x; b < N; b += kRowsPerWg)
+      s_end[b] = static_cast<uint32_t>(a.row_starts[min(b + 1, p.requests)]);
+    __syncthreads();
   }
+  const int r = blockIdx.x * kRowsPerWg + threadIdx.x;
+  if (r >= n_rows) return;
+  int b, t;
+  if (a.width > 0) {
+    b = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(a.width));
+    t = r - b * a.width;
+    if (t >= a.new_lens[b]) b = -1;
+  } else {
+    b = first_above<N>(s_end, static_cast<uint32_t>(r));
+    t = b < p.requests ? r - a.row_starts[b] : 0;
+    if (b >= p.requests) b = -1;
+  }
+  int64_t pos = 0, slot = -1;
+  if (b >= 0) {
+    pos = static_cast<int64_t>(a.starts[b]) + t;
+    if (a.granted[b] > 0)
+      slot = (static_cast<int64_t>(p.page_table[b * p.table_stride + (pos >> a.shift)]) << a.shift) +
+             (pos & ((1 << a.shift) - 1));
+  }
+  put_row(a, r, b, pos, slot);
 }
 
 // keep_lens: pages behind the kept lengths go back, the last ones first.
@@ -186,6 +251,7 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const ReleaseArgs
   __shared__ uint32_t s_wave[kPlanThreads / 64];
   __shared__ uint32_t s_upto[kPlanThreads * ITEMS];
   __shared__ int32_t s_at[kPlanThreads * ITEMS];
+  constexpr int kSide = side<ITEMS>();
   const fdllm_page_pool& p = a.pool;
   const int tid = threadIdx.x;
   const uint32_t count = static_cast<uint32_t>(min(max(*p.free_count, 0), p.num_free));
@@ -215,9 +281,16 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const ReleaseArgs
     s_upto[tid * ITEMS + k] = c;
   }
   __syncthreads();
-  for (uint32_t i = tid; i < n; i += kPlanThreads) {
-    const int b = first_above(s_upto, p.requests, i);
-    p.free_pages[count + n - 1 - i] = p.page_table[b * p.table_stride + static_cast<int32_t>(s_at[b] + i)];
+  for (uint32_t i0 = tid; i0 < n; i0 += kSide * kPlanThreads) {
+    int page[kSide];
+#pragma unroll
+    for (int k = 0; k < kSide; ++k) {
+      const uint32_t i = min(i0 + k * kPlanThreads, n - 1);  // the last one may be written twice
+      const int b = first_above<kPlanThreads * ITEMS>(s_upto, i);
+      page[k] = p.page_table[b * p.table_stride + static_cast<int32_t>(s_at[b] + i)];
+    }
+#pragma unroll
+    for (int k = 0; k < kSide; ++k) p.free_pages[count + n - 1 - min(i0 + k * kPlanThreads, n - 1)] = page[k];
   }
   if (tid == 0) *p.free_count = static_cast<int32_t>(count + n);
 }
@@ -245,9 +318,9 @@ extern "C" int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* ne
   using namespace fdllm;
   const char* what = "fdllm_assign_pages";
   if (const int rc = check_pool(what, pool)) return rc;
-  FDLLM_CHECK_ARG(width >= 0 && rows >= 0 && (width == 0 || rows == 0),
+  FDLLM_CHECK_ARG(width >= 0 && rows >= 0 && (width > 0) != (rows > 0),
                   "%s: give the padded form's width or the packed form's rows", what);
-  if (pool->requests == 0 && (width > 0 || rows == 0)) return FDLLM_OK;
+  if (pool->requests == 0 && width > 0) return FDLLM_OK;
   FDLLM_CHECK_ARG(pool->requests > 0, "%s: a packed list without requests", what);
   FDLLM_CHECK_ARG(new_lens && slots && positions && starts && seqlens && granted && (width > 0 || (sequences && row_starts)),
                   "%s: null pointer", what);
@@ -264,14 +337,22 @@ extern "C" int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* ne
   a.starts = starts;
   a.seqlens = seqlens;
   a.granted = granted;
-  const int64_t n_rows = width > 0 ? static_cast<int64_t>(width) * pool->requests : rows;
+  const int64_t all_rows = width > 0 ? static_cast<int64_t>(width) * pool->requests : rows;
+  FDLLM_CHECK_ARG(all_rows <= 0x7fffffff - kRowsPerWg, "%s: too many rows", what);
+  const int n_rows = static_cast<int>(all_rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (pool->requests <= kPlanThreads) assign_plan_kernel<1><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
-  else assign_plan_kernel<kMaxRequests / kPlanThreads><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
-  if (n_rows > 0) {
-    const int64_t wgs = (n_rows + 255) / 256;
-    assign_rows_kernel<<<dim3(static_cast<unsigned>(wgs < 2048 ? wgs : 2048)), dim3(256), 0, s>>>(a, n_rows);
+  const int B = pool->requests, T = kPlanThreads;
+  if (B <= 2 * T && n_rows <= kOneKernelRows) {
+    if (B <= T) assign_plan_kernel<1, true><<<dim3(1), dim3(T), 0, s>>>(a, n_rows);
+    else assign_plan_kernel<2, true><<<dim3(1), dim3(T), 0, s>>>(a, n_rows);
+    FDLLM_RETURN_LAUNCH_STATUS(what);
   }
+  if (B <= T) assign_plan_kernel<1, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
+  else if (B <= 2 * T) assign_plan_kernel<2, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
+  else assign_plan_kernel<kMaxRequests / T, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
+  const dim3 grid(static_cast<unsigned>((n_rows + kRowsPerWg - 1) / kRowsPerWg));
+  if (width > 0 || B <= T) assign_rows_kernel<T><<<grid, dim3(kRowsPerWg), 0, s>>>(a, n_rows);
+  else assign_rows_kernel<kMaxRequests><<<grid, dim3(kRowsPerWg), 0, s>>>(a, n_rows);
   FDLLM_RETURN_LAUNCH_STATUS(what);
 }
 
@@ -284,6 +365,7 @@ extern "C" int fdllm_release_pages(const fdllm_page_pool* pool, const int32_t* k
   ReleaseArgs a{*pool, keep_lens, __builtin_ctz(static_cast<unsigned>(pool->page_size))};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (pool->requests <= kPlanThreads) release_kernel<1><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
+  else if (pool->requests <= 2 * kPlanThreads) release_kernel<2><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
   else release_kernel<kMaxRequests / kPlanThreads><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
   FDLLM_RETURN_LAUNCH_STATUS(what);
 }

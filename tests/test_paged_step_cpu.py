@@ -132,6 +132,7 @@ def test_c_abi_refuses_bad_pools(lib):
         assert lib.fdllm_release_pages(ctypes.byref(pool(**kw)), 16, None) == bad, kw
     assert assign(None) == bad and lib.fdllm_release_pages(None, 16, None) == bad
     assert assign(pool(), 1, 1) == bad and assign(pool(), -1) == bad and assign(pool(), 0, -1) == bad
+    assert assign(pool(), 0, 0, 16) == bad and assign(pool(), 2 ** 30) == bad and assign(pool(), 0, 2 ** 31 - 1, 16) == bad
     assert assign(pool(), 0, 4) == bad  # the packed form without its two outputs
     assert assign(pool(requests=0), 0, 4, 16) == bad
     assert assign(pool(requests=0)) == 0 and lib.fdllm_release_pages(ctypes.byref(pool(requests=0)), None, None) == 0
