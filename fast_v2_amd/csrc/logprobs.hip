@@ -55,7 +55,7 @@ struct ScoreArgs {
   float* top_logprobs;
   int64_t* top_tokens;
   int splits, steps;  // workgroups per row, steps of each
-  float* parts;       // splits > 1: [rows][splits] of float4 (m, S, A, -), then [rows][n_groups] maxima
+  float* parts;       // splits > 1: [rows][splits][waves] of float4 (m, S, A, -), then [rows][n_groups] maxima
   int n_groups;
   int64_t rows;
 };
@@ -131,25 +131,30 @@ __device__ __forceinline__ void wave_sync() {
 struct State {
   float m, s, a;
 };
+// e^t, as 2^(t log2 e) with the constant in one part
+__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t * 1.44269504f); }
 // the state relative to another maximum to >= m
 __device__ __forceinline__ void rescale(State& x, float to) {
   if (x.m == to) return;
   const float d = x.m == -INFINITY ? 0.f : x.m - to;
-  const float e = expf(d);
+  const float e = exp_of(d);
   x.a = e * __builtin_fmaf(fmaxf(d, -1e30f), x.s, x.a);  // e is 0 long before that bound: 0 times -inf is not 0
   x.s *= e;
   x.m = to;
 }
 
-// Joins the workgroup's states; every thread returns with the row's.
-template <int NW>
-__device__ __forceinline__ State join(State x, float* s_red) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float mw = wave_allreduce_max(x.m);
-  rescale(x, mw);
+// Joins a wave's states.
+__device__ __forceinline__ State join_wave(State x) {
+  rescale(x, wave_allreduce_max(x.m));
   x.s = wave_allreduce_sum(x.s);
   x.a = wave_allreduce_sum(x.a);
-  if (lane == 0) {
+  return x;
+}
+// Joins the waves' states; every thread returns with the workgroup's.
+template <int NW>
+__device__ __forceinline__ State join(const State& x, float* s_red) {
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
     s_red[3 * wave] = x.m;
     s_red[3 * wave + 1] = x.s;
     s_red[3 * wave + 2] = x.a;
@@ -159,7 +164,7 @@ __device__ __forceinline__ State join(State x, float* s_red) {
 #pragma unroll
   for (int w = 1; w < NW; ++w) m = fmaxf(m, s_red[3 * w]);
   State r{m, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
   for (int w = 0; w < NW; ++w) {
     State y{s_red[3 * w], s_red[3 * w + 1], s_red[3 * w + 2]};
     rescale(y, m);
@@ -397,7 +402,7 @@ __global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
   const int64_t r = row;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const RowVecs rv = row_of<T>(a, row);
-  float* groups = a.parts + a.rows * a.splits * 4 + r * a.n_groups;  // splits > 1
+  float* groups = a.parts + a.rows * a.splits * (4 * kWaves) + r * a.n_groups;  // splits > 1
   State st{-INFINITY, 0.f, 0.f};
   Given given{false, 0.f};
   if (a.splits == 1) given = given_of<T>(a, r, threadIdx.x, rv);
@@ -432,7 +437,7 @@ __global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float t = x[u][j] - ref;
-        const float e = __builtin_amdgcn_exp2f(t * 1.44269504f);
+        const float e = exp_of(t);
         st.s += e;
         st.a = __builtin_fmaf(e, fmaxf(t, -1e30f), st.a);  // a banned token's 0 times -inf counts as 0
       }
@@ -449,11 +454,12 @@ __global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
       }
     }
   }
-  st = join<kWaves>(st, sh.red);  // a barrier: the group maxima are in LDS after it
+  st = join_wave(st);
   if (a.splits == 1) {
+    st = join<kWaves>(st, sh.red);  // a barrier: the group maxima are in LDS after it
     finish<T, kThreads>(a, r, rv, st, given, sh);
-  } else if (threadIdx.x == 0) {
-    reinterpret_cast<float4*>(a.parts)[blockIdx.x] = make_float4(st.m, st.s, st.a, 0.f);
+  } else if (lane == 0) {  // each wave's own: the finish folds them
+    reinterpret_cast<float4*>(a.parts)[blockIdx.x * static_cast<int64_t>(kWaves) + wave] = make_float4(st.m, st.s, st.a, 0.f);
   }
 }
 
@@ -464,10 +470,11 @@ __global__ __launch_bounds__(kFinishThreads) void score_finish_kernel(const Scor
   const RowVecs rv = row_of<T>(a, blockIdx.x);
   const int tid = threadIdx.x;
   // what is read of the row: the workgroups' states by the first wave, the groups' maxima by all
-  const float4* parts = reinterpret_cast<const float4*>(a.parts) + r * a.splits;
-  const float* groups = a.parts + a.rows * a.splits * 4 + r * a.n_groups;
+  const int np = a.splits * kWaves;
+  const float4* parts = reinterpret_cast<const float4*>(a.parts) + r * np;
+  const float* groups = a.parts + a.rows * np * 4 + r * a.n_groups;
   float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  if (tid < a.splits) p = parts[tid];
+  if (tid < np) p = parts[tid];
   if (a.top > 0) {
 #pragma unroll 1
     for (int g = tid; g < a.n_groups; g += kFinishThreads) sh.group[g] = groups[g];
@@ -476,7 +483,7 @@ __global__ __launch_bounds__(kFinishThreads) void score_finish_kernel(const Scor
   if (tid < 64) {
     State st{p.x, p.y, p.z};
 #pragma unroll 1
-    for (int s = tid + 64; s < a.splits; s += 64) {
+    for (int s = tid + 64; s < np; s += 64) {
       const float4 q = parts[s];
       State y{q.x, q.y, q.z};
       const float m = fmaxf(st.m, y.m);
@@ -485,10 +492,10 @@ __global__ __launch_bounds__(kFinishThreads) void score_finish_kernel(const Scor
       st.s += y.s;
       st.a += y.a;
     }
-    rescale(st, wave_allreduce_max(st.m));
+    st = join_wave(st);
     sh.red[0] = st.m;
-    sh.red[1] = wave_allreduce_sum(st.s);
-    sh.red[2] = wave_allreduce_sum(st.a);
+    sh.red[1] = st.s;
+    sh.red[2] = st.a;
   }
   __syncthreads();
   finish<T, kFinishThreads>(a, r, rv, State{sh.red[0], sh.red[1], sh.red[2]}, given, sh);
@@ -509,7 +516,7 @@ Cut cut(int vocab, int64_t rows, int dtype) {
   const int64_t splits = want < all ? want : all;
   c.steps = static_cast<int>((all + splits - 1) / splits);
   c.splits = static_cast<int>((all + c.steps - 1) / c.steps);
-  c.bytes = c.splits > 1 ? (static_cast<size_t>(rows) * c.splits * 4 + static_cast<size_t>(rows) * c.n_groups) * 4 : 0;
+  c.bytes = c.splits > 1 ? (static_cast<size_t>(rows) * c.splits * (4 * kWaves) + static_cast<size_t>(rows) * c.n_groups) * 4 : 0;
   return c;
 }
 
