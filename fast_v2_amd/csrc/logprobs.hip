@@ -126,18 +126,30 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The sums in powers of two: u = x log2 e - R with R = m log2 e rounded, one fused operation a logit;
+// S = sum 2^u, A = sum u 2^u. That R is not m log2 e to the last bit does not matter, as long as
+// every use takes the same one. Where it could overflow (a maximum near the type's largest or
+// lowest value) u = (x - m) log2 e.
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr float kLargeMax = 1e37f;
+__device__ __forceinline__ float powers_above(float x, float m) {  // u
+  return fabsf(m) < kLargeMax ? __builtin_fmaf(x, kLog2e, -(m * kLog2e)) : (x - m) * kLog2e;
+}
+
 // S and A relative to the maximum m. While nothing above -inf was read they are 0, or NaN
 // after a NaN logit, which then stays.
 struct State {
   float m, s, a;
 };
-// e^t, as 2^(t log2 e) with the constant in one part
-__device__ __forceinline__ float exp_of(float t) { return __builtin_amdgcn_exp2f(t * 1.44269504f); }
-// the state relative to another maximum to >= m
+// the state relative to another maximum to >= m: S' = 2^d S, A' = 2^d (A + d S)
 __device__ __forceinline__ void rescale(State& x, float to) {
   if (x.m == to) return;
-  const float d = x.m == -INFINITY ? 0.f : x.m - to;
-  const float e = exp_of(d);
+  float d = 0.f;
+  if (x.m != -INFINITY) {
+    const bool small = fabsf(x.m) < kLargeMax && fabsf(to) < kLargeMax;
+    d = small ? x.m * kLog2e - to * kLog2e : (x.m - to) * kLog2e;
+  }
+  const float e = __builtin_amdgcn_exp2f(d);
   x.a = e * __builtin_fmaf(fmaxf(d, -1e30f), x.s, x.a);  // e is 0 long before that bound: 0 times -inf is not 0
   x.s *= e;
   x.m = to;
@@ -211,35 +223,37 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return ((b >> 31) ? ~b : b | 0x80000000u) - 0x007fffffu;
 }
 
-// A row's alternatives, by NT threads; sh.group holds its groups' maxima. The code runs once a row, so
-// its own loading counts: no loop is unrolled that need not be.
+// Into sh.bound a bound that K logits reach, by one wave: the K-th of 64 maxima, each over the groups
+// that a lane takes. Clears the counters of what follows.
+template <typename T, int NT>
+__device__ __forceinline__ void find_bound(const ScoreArgs& a, int lane, Shared<T, NT>& sh) {
+  float mine = -INFINITY;
+#pragma unroll 2
+  for (int g = lane; g < a.n_groups; g += 64) mine = fmaxf(mine, sh.group[g]);
+  sh.lane_max[lane] = mine;
+  wave_sync();
+  int above = 0;
+#pragma unroll 2
+  for (int h = 0; h < 64; h += 4) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(&sh.lane_max[h]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) above += y[j] > mine;
+  }
+  const float m = -wave_allreduce_max(above < a.top ? -mine : -INFINITY);  // the least that fewer than K exceed
+  if (lane < 33) sh.n_above[lane] = 0;
+  if (lane == 0) {
+    sh.bound = m;
+    sh.n_sel = sh.n_cand = 0;
+  }
+}
+
+// A row's alternatives, by NT threads; sh.group holds its groups' maxima, sh.bound the bound. The code
+// runs once a row, so its own loading counts: no loop is unrolled that need not be.
 template <typename T, int NT, typename Put>
 __device__ __forceinline__ void alternatives(const ScoreArgs& a, const RowVecs& rv, Put put, Shared<T, NT>& sh) {
   constexpr int N = Vec<T>::N;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int K = a.top, ng = a.n_groups;
-  // a bound that K logits reach: the K-th of 64 maxima, each over the groups that a lane takes
-  if (wave == 0) {
-    float mine = -INFINITY;
-#pragma unroll 2
-    for (int g = lane; g < ng; g += 64) mine = fmaxf(mine, sh.group[g]);
-    sh.lane_max[lane] = mine;
-    wave_sync();
-    int above = 0;
-#pragma unroll 2
-    for (int h = 0; h < 64; h += 4) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(&sh.lane_max[h]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) above += y[j] > mine;
-    }
-    const float m = -wave_allreduce_max(above < K ? -mine : -INFINITY);  // the least that fewer than K exceed
-    if (lane < 33) sh.n_above[lane] = 0;
-    if (lane == 0) {
-      sh.bound = m;
-      sh.n_sel = sh.n_cand = 0;
-    }
-  }
-  __syncthreads();
   const float bound = sh.bound;
   // the groups that hold a logit from the bound up
 #pragma unroll 1
@@ -350,19 +364,23 @@ __device__ __forceinline__ void finish(const ScoreArgs& a, int64_t r, const RowV
   const int tid = threadIdx.x;
   // a NaN or +inf logit makes the sum NaN, a row without a finite one leaves it 0
   const bool good = st.s > 0.f;
-  const float lse = logf(st.s);
+  const float log2s = __builtin_amdgcn_logf(st.s);
   const float nan = __builtin_nanf("");
-  if (tid == 0) a.entropy[r] = good ? lse - st.a / st.s : nan;
+  // log p = x - m - log of the sum relative to m itself, which R is off from
+  const float off = fabsf(st.m) < kLargeMax ? __builtin_fmaf(st.m, kLog2e, -(st.m * kLog2e)) : 0.f;
+  const float lse = (log2s - off) * kLn2;
+  auto logp = [&](float x) __attribute__((always_inline)) { return x - st.m - lse; };
+  if (tid == 0) a.entropy[r] = good ? (log2s - st.a / st.s) * kLn2 : nan;
 #pragma unroll 1
   for (int j = tid; j < a.given; j += NT) {
-    a.logprobs[r * a.given + j] = good && g.in ? g.x - st.m - lse : nan;
+    a.logprobs[r * a.given + j] = good && g.in ? logp(g.x) : nan;
     g = given_of<T>(a, r, j + NT, rv);
   }
   const int K = a.top;
   if (good && K > 0) {  // uniform
     alternatives<T, NT>(a, rv, [&](int k, float v, int i) __attribute__((always_inline)) {
       a.top_tokens[r * K + k] = i;
-      a.top_logprobs[r * K + k] = v - st.m - lse;
+      a.top_logprobs[r * K + k] = logp(v);
     }, sh);
   } else if (tid < K) {
     a.top_tokens[r * K + tid] = -1;
@@ -394,13 +412,13 @@ __device__ __forceinline__ void group_maxima(float* m, int lane) {
 
 // One workgroup per row, or per `steps` steps of a row that several share.
 template <typename T>
-__global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
+__global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
   constexpr int N = Vec<T>::N, U = kStep / kWaves / Vec<T>::kGroup;  // a lane's vectors in a step
   __shared__ Shared<T, kThreads> sh;
   const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.splits);
   const int split = static_cast<int>(blockIdx.x - row * a.splits);
   const int64_t r = row;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const RowVecs rv = row_of<T>(a, row);
   float* groups = a.parts + a.rows * a.splits * (4 * kWaves) + r * a.n_groups;  // splits > 1
   State st{-INFINITY, 0.f, 0.f};
@@ -411,20 +429,23 @@ __global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
     const int g = ((split * a.steps + k) * kWaves + wave) * U;
     const int v0 = g * 64 + lane;
     if (g >= a.n_groups) break;  // uniform over the wave
-    u32x4 w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v0 + 64 * u < rv.nv) w[u] = __builtin_nontemporal_load(rv.v + v0 + 64 * u);
+    const int e0 = g * Vec<T>::kGroup - rv.mis;
     float x[U][N], mu[U];
+    u32x4 w[U];
+    if (e0 >= 0 && e0 + U * Vec<T>::kGroup <= a.V) {  // uniform: all of them are the row's
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = __builtin_nontemporal_load(rv.v + v0 + 64 * u);
+#pragma unroll
+      for (int u = 0; u < U; ++u) Vec<T>::get(w[u], x[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = rv.v[min(v0 + 64 * u, rv.nv - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u) unpack<T>(w[u], v0 + 64 * u, rv, a.V, x[u]);  // -inf past the row's end
+    }
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (v0 + 64 * u < rv.nv) {
-        unpack<T>(w[u], v0 + 64 * u, rv, a.V, x[u]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[u][j] = -INFINITY;
-      }
       mu[u] = x[u][0];
 #pragma unroll
       for (int j = 1; j < N; ++j) mu[u] = fmaxf(mu[u], x[u][j]);
@@ -432,15 +453,29 @@ __global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
     }
     if (m > st.m) rescale(st, m);
     const float ref = st.m == -INFINITY ? 0.f : st.m;
+    // a banned token's 0 times -inf counts as 0
+    if (__builtin_amdgcn_ballot_w64(fabsf(ref) >= kLargeMax) == 0) {
+      const float r2 = ref * kLog2e;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float t = x[u][j] - ref;
-        const float e = exp_of(t);
-        st.s += e;
-        st.a = __builtin_fmaf(e, fmaxf(t, -1e30f), st.a);  // a banned token's 0 times -inf counts as 0
-      }
+        for (int j = 0; j < N; ++j) {
+          const float t = __builtin_fmaf(x[u][j], kLog2e, -r2);
+          const float e = __builtin_amdgcn_exp2f(t);
+          st.s += e;
+          st.a = __builtin_fmaf(e, fmaxf(t, -1e30f), st.a);
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float t = powers_above(x[u][j], ref);
+          const float e = __builtin_amdgcn_exp2f(t);
+          st.s += e;
+          st.a = __builtin_fmaf(e, fmaxf(t, -1e30f), st.a);
+        }
+    }
     if (a.top > 0) {
       group_maxima<U>(mu, lane);
       const int u0 = (lane >> 5) * (U / 2) + ((lane >> 4) & 1) * (U / 4);
@@ -457,6 +492,10 @@ __global__ __launch_bounds__(kThreads, 8) void score_kernel(const ScoreArgs a) {
   st = join_wave(st);
   if (a.splits == 1) {
     st = join<kWaves>(st, sh.red);  // a barrier: the group maxima are in LDS after it
+    if (a.top > 0) {
+      if (wave == 0) find_bound<T, kThreads>(a, lane, sh);
+      __syncthreads();
+    }
     finish<T, kThreads>(a, r, rv, st, given, sh);
   } else if (lane == 0) {  // each wave's own: the finish folds them
     reinterpret_cast<float4*>(a.parts)[blockIdx.x * static_cast<int64_t>(kWaves) + wave] = make_float4(st.m, st.s, st.a, 0.f);
@@ -468,22 +507,25 @@ __global__ __launch_bounds__(kFinishThreads) void score_finish_kernel(const Scor
   __shared__ Shared<T, kFinishThreads> sh;
   const int64_t r = blockIdx.x;
   const RowVecs rv = row_of<T>(a, blockIdx.x);
-  const int tid = threadIdx.x;
-  // what is read of the row: the workgroups' states by the first wave, the groups' maxima by all
+  const int tid = threadIdx.x, lane = tid & 63;
+  // what is read of the row: the waves' states by the second wave, the groups' maxima by all
   const int np = a.splits * kWaves;
   const float4* parts = reinterpret_cast<const float4*>(a.parts) + r * np;
   const float* groups = a.parts + a.rows * np * 4 + r * a.n_groups;
   float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-  if (tid < np) p = parts[tid];
+  if (tid >> 6 == 1 && lane < np) p = parts[lane];
   if (a.top > 0) {
 #pragma unroll 1
     for (int g = tid; g < a.n_groups; g += kFinishThreads) sh.group[g] = groups[g];
   }
   const Given given = given_of<T>(a, r, tid, rv);
-  if (tid < 64) {
+  __syncthreads();
+  if (tid >> 6 == 0) {
+    if (a.top > 0) find_bound<T, kFinishThreads>(a, lane, sh);
+  } else if (tid >> 6 == 1) {
     State st{p.x, p.y, p.z};
 #pragma unroll 1
-    for (int s = tid + 64; s < np; s += 64) {
+    for (int s = lane + 64; s < np; s += 64) {
       const float4 q = parts[s];
       State y{q.x, q.y, q.z};
       const float m = fmaxf(st.m, y.m);
