@@ -555,6 +555,8 @@ fdllm_page_pool page_pool(PyObject* const* a, const Tensor& ask) {
   plain(B > 0 && B <= INT32_MAX && most <= INT32_MAX && lens.size(0) == B && ask.size(0) == B && page > 0 &&
         page <= INT32_MAX && pages.size(0) <= INT32_MAX && (most == 0 || table.stride(1) == 1) &&
         (B == 1 || table.stride(0) >= most));
+  const char *x = static_cast<const char*>(ask.data_ptr()), *y = static_cast<const char*>(lens.data_ptr());
+  plain(x + 4 * B <= y || y + 4 * B <= x);  // read after the lengths have changed
   on_current_device(lens);
   fdllm_page_pool p;
   p.page_table = static_cast<int32_t*>(table.data_ptr());

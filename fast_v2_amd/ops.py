@@ -896,10 +896,18 @@ def kv_cache_write(
 _INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 
 
-def _no_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Inference calls: a tensor to differentiate is refused, its gradient would be lost."""
+def _inference(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses what a kernel would read wrongly or drop: tensors to differentiate (there is no
+    backward pass), subclasses, transforms' wrappers, pending negations, tangents."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what}: no backward pass (call it under torch.no_grad(), or detach the tensors)")
+    if not _plain_tensors(*tensors):
+        raise RuntimeError(f"{what}: plain tensors expected (no subclass, function transform, pending negation or tangent)")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
 
 
 def _launching(dev: torch.device):
@@ -931,6 +939,7 @@ class PageRows(NamedTuple):
 
 def _page_pool(what, lens, page_table, free_pages, free_count, page_size, *more):
     dev = _require_gpu(lens, page_table, free_pages, free_count, *more)
+    _inference(what, lens, page_table, free_pages, free_count, *more)
     if any(t.dtype != torch.int32 for t in (lens, page_table, free_pages, free_count)):
         raise RuntimeError(f"{what}: lens, page_table, free_pages and free_count must be int32 (changed in place)")
     if page_table.dim() != 2 or lens.shape != page_table.shape[:1] or free_pages.dim() != 1 or free_count.numel() != 1:
@@ -977,6 +986,8 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.T
     if new_lens.shape != lens.shape:
         raise RuntimeError(f"{what}: new_lens must be [B]")
     new_lens = _int32(what, new_lens)
+    if _overlap(new_lens, lens):  # read after the lengths have grown
+        new_lens = new_lens.clone()
     B = p.requests
     shape = (B, width) if width else (rows,)
     slots = torch.empty(shape, dtype=torch.int64, device=dev)
@@ -1007,6 +1018,8 @@ def release_pages(keep_lens: torch.Tensor, lens: torch.Tensor, page_table: torch
     if keep_lens.shape != lens.shape:
         raise RuntimeError(f"{what}: keep_lens must be [B]")
     keep_lens = _int32(what, keep_lens)
+    if _overlap(keep_lens, lens):
+        keep_lens = keep_lens.clone()
     with _launching(dev):
         rc = _ffi.lib().fdllm_release_pages(ctypes.byref(p), keep_lens.data_ptr(), _ffi.stream_ptr(dev))
     _ffi.check(rc, "fdllm_release_pages")
@@ -1070,7 +1083,8 @@ def norm_rope_kv_write(
     q_weight, k_weight  [D] of the norms (the heads' dtype or fp32); None: that one is not normed
     k_cache, v_cache    [num_pages, page_size, Hkv, D] pools in any strides of whole 16-byte
                rows (``block_attn``'s); written in place at ``slots`` [B, S] (page * page_size +
-               offset; rows outside of the pool, as -1, are not written; repeated slots race)
+               offset; rows outside of the pool, as -1, are not written; repeated slots race);
+               apart from each other and from q, k, v
     interleaved  pairs are (2 i, 2 i + 1) in place of (i, i + R / 2)
 
     Held in fp32 (angles in 64 bits) and rounded once. Returns the new queries [B, S, Hq, D],
@@ -1090,7 +1104,7 @@ def norm_rope_kv_write(
         raise RuntimeError(f"{what}: give k_cache, v_cache and slots together")
     given = [t for t in (positions, inv_freq, q_weight, k_weight, k_cache, v_cache, slots) if t is not None]
     dev = _require_gpu(q, k, v, *given)
-    _no_grad(what, q, k, v, inv_freq, q_weight, k_weight, k_cache, v_cache)
+    _inference(what, q, k, v, positions, inv_freq, q_weight, k_weight, k_cache, v_cache, slots)
     if q.dtype not in (torch.bfloat16, torch.float16, torch.float32) or \
             any(t is not None and t.dtype != q.dtype for t in (k, v, k_cache, v_cache)):
         raise RuntimeError(f"{what}: q, k, v and the caches must share bf16, fp16 or fp32")
@@ -1185,7 +1199,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if logits.dim() < 1 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise RuntimeError(f"{what}: logits [..., V] in bf16, fp16 or fp32 expected")
     dev = _require_gpu(logits, *([tokens] if tokens is not None else []))
-    _no_grad(what, logits)
+    _inference(what, logits, tokens)
     lead, V = logits.shape[:-1], logits.shape[-1]
     top_k = int(top_k)
     if not 0 <= top_k <= min(32, V):

@@ -151,6 +151,27 @@ def test_bad_numbers_stay_in_their_rows(gpu):
     assert (ops.norm_rope_kv_write(q, k, v, pos, freq, w, w) == 0).all()
 
 
+@pytest.mark.parametrize("head_major", [False, True])
+def test_pools_past_32_bits(gpu, head_major):
+    """Rows at the end of pools of more than 2^31 elements, and at their start."""
+    Hkv, D, page = 4, 128, 32
+    pages = 2 ** 31 // (page * Hkv * D) + 7
+    q, k, v = _inputs(gpu, 1, 6, 4, Hkv, D, BF16, 12)
+    pos = torch.arange(6, dtype=torch.int32, device=gpu)[None]
+    last = pages * page
+    slots = torch.tensor([[last - 1, 0, last, last - 40, 2 ** 31 // (Hkv * D) + 1, 1]], device=gpu)
+    shape = (pages, Hkv, page, D) if head_major else (pages, page, Hkv, D)
+    pools = [torch.zeros(shape, dtype=BF16, device=gpu) for _ in range(2)]
+    views = [p.transpose(1, 2) if head_major else p for p in pools]
+    freq = ops.rope_frequencies(D)[0].to(gpu)
+    _, k_got = ops.norm_rope_kv_write(q, k, v, pos, freq, k_cache=views[0], v_cache=views[1], slots=slots, kv_out=True)
+    for c, rows in zip(views, (k_got, v)):
+        for t, s in enumerate(slots[0].tolist()):
+            if s < last:
+                assert torch.equal(c[s // page, s % page], rows[0, t]), t
+        assert int((c != 0).any(-1).any(-1).sum()) == 5
+
+
 def test_empty(gpu):
     f = ops.rope_frequencies(64)[0].to(gpu)
     for B, S in ((0, 4), (3, 0)):

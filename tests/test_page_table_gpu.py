@@ -117,6 +117,18 @@ def test_numbers_at_their_limits(gpu):
     pool.assign([big, -big, 2, 0, 0], width=8, as_given=new)
 
 
+def test_large_page_ids(gpu):
+    """Slots past 32 bits: page ids near their type's end."""
+    rng = np.random.default_rng(10)
+    pool = _Pool(gpu, [70, 0, 64], 4, 64, 5, rng)
+    far = 2 ** 31 - 1 - np.arange(pool.size)
+    pool.free = far[:len(pool.free)].tolist()
+    pool.g_free[:len(pool.free)] = torch.tensor(pool.free, dtype=torch.int32, device=gpu)
+    got, want = pool.assign([100, 1, 1], rows=102)
+    assert got.slots.max() > 2 ** 36
+    pool.release([0, 0, 0])
+
+
 def test_no_pages_no_room(gpu):
     rng = np.random.default_rng(6)
     pool = _Pool(gpu, [30, 32, 0], 2, 32, 0, rng)

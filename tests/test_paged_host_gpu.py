@@ -18,7 +18,7 @@ def _pool():
 
 
 @pytest.mark.parametrize("form", ["padded", "packed", "int64", "wide_table", "one", "strided_lens", "float", "shape",
-                                  "neither", "page", "cpu"])
+                                  "neither", "page", "cpu", "itself"])
 def test_pages(gpu, form):
     print(f"case pages {form}", flush=True)
 
@@ -43,15 +43,17 @@ def test_pages(gpu, form):
             pool[4] = 24
         elif form == "cpu":
             pool[2] = pool[2].cpu()
+        elif form == "itself":  # as many again as there are
+            new = pool[0]
 
         def fn():
             out = ops.assign_pages(new, *pool, **kw)
-            keep = out.starts.long() if form == "int64" else out.starts
+            keep = out.starts.long() if form == "int64" else pool[0] if form == "itself" else out.starts
             assert ops.release_pages(keep, *pool) is None
             return out
         return fn, pool
     left = {"int64": ("assign", "release"), "strided_lens": ("assign",), "float": ("assign",), "shape": ("assign",),
-            "neither": ("assign",), "cpu": ("assign",)}
+            "neither": ("assign",), "cpu": ("assign",), "itself": ("assign", "release")}
     _same(*_both(make, left.get(form, ())))
 
 
@@ -213,3 +215,27 @@ def test_inference_mode_and_wrappers(gpu):
         return t
     torch.vmap(fn)(_rnd(1, 3, 2, 50))
     assert seen == [None]
+
+
+def test_wrapped_tensors_are_refused(gpu):
+    """What carries more than its values: refused, not read without it."""
+    import torch.autograd.forward_ad as fwd
+
+    class Sub(torch.Tensor):
+        pass
+    x, i = _rnd(1, 1, 1, 2, 8), torch.zeros(1, 1, **I32)
+    f = torch.ones(4, device="cuda")
+    neg = torch._neg_view(x)
+    assert neg.is_neg()
+    for bad in (x.as_subclass(Sub), neg):
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            ops.token_logprobs(bad)
+        with pytest.raises(RuntimeError):
+            ops.norm_rope_kv_write(bad, x, x, i, f)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            ops.token_logprobs(fwd.make_dual(x.float(), x.float()))
+    pool = list(_pool())
+    pool[1] = pool[1].as_subclass(Sub)
+    with pytest.raises(RuntimeError, match="plain tensors"):
+        ops.assign_pages(torch.ones(3, **I32), *pool, width=1)
