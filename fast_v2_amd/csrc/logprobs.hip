@@ -4,10 +4,10 @@
 //   m = max x,  S = sum e^(x - m),  A = sum (x - m) e^(x - m)
 //   log p(t) = x_t - m - log S,     H = -sum p log p = log S - A / S
 //
-// Each thread holds (m, S, A) of the logits it has read and rescales when its maximum grows
-// (e^d with d = m - m': S' = e^d S, A' = e^d (A + d S)); states of threads, and of workgroups
-// that share a long row, are joined by the same rule. All in fp32: (x - m) is exact for 16-bit
-// logits near m, and the sums are trees of at most 2^-24 relative error a level.
+// Each thread holds (m, S, A) of the logits it has read, S and A in powers of two, and rescales when its
+// maximum grows (2^d with d = (m - m') log2 e: S' = 2^d S, A' = 2^d (A + d S)); states of threads, and of
+// workgroups that share a long row, are joined by the same rule, in an order that is always the same. All in
+// fp32: the sums are short chains (32 logits a step) under trees, each addition off by at most 2^-24.
 //
 // Alternatives without keeping a list while reading: the pass leaves the maximum of every
 // group of neighbouring logits that a wave loads at once (64 vectors of 16 bytes). The K-th of 64
@@ -18,14 +18,13 @@
 // values, then the logits above it are ranked and its first equals fill up.
 //
 // What bounds it: many rows, the one read of the logits beside the vector units: 4 x 512 rows of 152064
-// bf16 logits (623 MB) 118 us, 5.3 TB/s, where a plain read of the memory takes 99; ten operations and an
-// exponential a logit take about 85 us of every SIMD. (x - m) log2 e is one product: the constant in two parts (a
-// multiply-add more) takes 2.4 us more and the results are no nearer to 64 bits (5.8e-8 both). Few rows, latency:
-// one fp32 row 11 us, 16 x 8 bf16 rows 17 us, of which the finish is 5: its phases are states and maxima 1.4 us,
-// bound 1.2, groups 0.3, their logits 0.9, ranks 0.7. Its code runs once a row and is loaded for it, so
-// it is kept short: with loops unrolled the finish took 9 us (K = 5) to 19 (K = 20).
-#include <math.h>
-
+// bf16 logits (623 MB) 112 us, 5.6 TB/s, where a plain read of the memory takes 99. 9.6 vector instructions
+// a logit, one of them the exponential, are about 95 us of every SIMD (with edge checks in every step
+// and (x - m) log2 e as two operations 12 a logit and 117 us). The next step's loads ahead of this one's
+// arithmetic took 4 us more, as fewer waves fit. Few rows, latency: one fp32 row with 20 alternatives 9.5
+// us, 16 x 8 bf16 rows with 5 15.4 us, of which the finish is 5: states and maxima 0.9 us, bound 1.1, groups 0.3, their
+// logits 0.9, ranks 0.5, launch. Its code runs once a row and is loaded for it, so it is kept
+// short: with loops unrolled the finish took 9 us (K = 5) to 19 (K = 20).
 #include "fdllm_common.h"
 
 namespace fdllm {
@@ -36,8 +35,8 @@ constexpr int kWaves = kThreads / 64;
 // Threads of a row's finish: 256 take 0.9 us more for 20 alternatives of one fp32 row, 1024 1.3 us
 // more (2 to 5 us where there are many rows).
 constexpr int kFinishThreads = 512;
-// Workgroups that a call aims at: 1024 take 19.0 us for 16 x 8 rows of 152064, 2048 17.2, 4096 18.1
-// (more partials, one step each); from 2048 rows on a workgroup takes whole rows.
+// Workgroups that a call aims at: 1024 take 1.8 us more for 16 x 8 rows of 152064, 4096 0.9 us more (more
+// partials, one step each); from 2048 rows on a workgroup takes whole rows.
 constexpr int kWorkgroups = 2048;
 constexpr int kStep = 2048 * kWaves;      // logits of a workgroup's step
 constexpr int kMaxVocab = 1 << 20;

@@ -8,7 +8,7 @@ dtypes or a missing library raise ``RuntimeError``.
 torch.library ops (namespace ``fdllm``), each with a Meta implementation so
 that graph capture / FakeTensor tracing can infer output shapes without data,
 in the manner of ``_wrap_flash_kvcache_as_custom_op``
-(utils/attention_backends.py:73-120):
+(utils/attention_backends.py:73-120; the other functions launch directly):
 
     fdllm::flash_kvcache(Tensor q, Tensor k_cache, Tensor v_cache,
                          Tensor cache_seqlens, float softmax_scale, bool causal) -> Tensor

@@ -1,7 +1,7 @@
 /*
  * libfdllm_hip.so — C ABI of the MI355X (gfx950) block-diffusion hot path.
  *
- * Two operator families, each a drop-in for one surface of navneet-13/fast_v2:
+ * Three operator families; the first two are drop-ins for a surface of navneet-13/fast_v2:
  *
  *   1. Row gather + RMSNorm (and the sibling row scatter), replacing the
  *      pybind entry points of cuda_bench/fused_gather_norm.cu:215-221.
@@ -10,6 +10,9 @@
  *      AttentionBackend.flash_kvcache_attention (utils/attention_backends.py:588-640)
  *      and the eager block-causal SDPA of the prefill/commit forward
  *      (modeling.py:385-411 with eval_block_diff_mask, modeling.py:145-150).
+ *   3. A paged step's other ends (at the end of this file): pages, slots and positions of new
+ *      tokens from the requests' lengths; head norms, position rotation and the paged K / V
+ *      write; log probabilities, entropy and alternatives of the logits.
  *
  * Conventions shared by every entry point:
  *   - Plain device pointers, element strides and sizes; no framework types.

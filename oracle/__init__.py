@@ -15,6 +15,9 @@ Modules
                   RoPE, sub-block cache, static cache write, SDPA shim), plugged
                   into the generation loop for the end-to-end comparison
 
+  paged_step      pages and slots of new tokens, head norms + rotation, token log
+                  probabilities, from their definitions in include/fdllm_hip.h
+
 Pinning status (what checks each function; see tests/test_oracle_*.py):
   attention.sdpa_kvcache            pinned: fp64 brute force, committed golden
                                     vectors (torch CPU SDPA), closed forms
@@ -49,6 +52,11 @@ Pinning status (what checks each function; see tests/test_oracle_*.py):
                                     position 0, norms kept, relative positions).
                                     The projections are the model's own nn.Linear
                                     modules, applied in the reference's order
+  paged_step                        pinned: a page table by hand, pages that run out in
+                                    order, a step taken back; rotation against explicit
+                                    cos / sin, identity at position 0, unit RMS;
+                                    uniform, excluded and linear logits
+                                    (tests/test_paged_step_cpu.py)
 There are no golden vectors in the reference (its tests generate inputs from
 seeds on CUDA), and no function here needed an import of the reference.
 """
