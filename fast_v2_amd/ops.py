@@ -937,7 +937,14 @@ class PageRows(NamedTuple):
     row_starts: Optional[torch.Tensor]  # packed: int32 [requests + 1], where a request's rows begin
 
 
+def _sizes(what: str, *sizes: int) -> None:
+    """Refuses sizes past 32 bits, which the descriptors' fields would wrap."""
+    if max(sizes) > 2 ** 31 - 1:
+        raise RuntimeError(f"{what}: size {max(sizes)} is too large")
+
+
 def _page_pool(what, lens, page_table, free_pages, free_count, page_size, *more):
+    _sizes(what, page_size, *page_table.shape, *free_pages.shape)
     dev = _require_gpu(lens, page_table, free_pages, free_count, *more)
     _inference(what, lens, page_table, free_pages, free_count, *more)
     if any(t.dtype != torch.int32 for t in (lens, page_table, free_pages, free_count)):
@@ -982,6 +989,7 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.T
             return PageRows(*done)
     if (width > 0) == (rows > 0) or width < 0 or rows < 0:
         raise RuntimeError(f"{what}: give the padded form's width or the packed form's rows")
+    _sizes(what, rows, width * max(lens.numel(), 1))
     p, dev = _page_pool(what, lens, page_table, free_pages, free_count, page_size, new_lens)
     if new_lens.shape != lens.shape:
         raise RuntimeError(f"{what}: new_lens must be [B]")
@@ -1100,6 +1108,7 @@ def norm_rope_kv_write(
         raise RuntimeError(f"{what}: q [B, S, Hq, D], k / v [B, S, Hkv, D] expected")
     B, S, Hq, D = q.shape
     Hkv = k.shape[2]
+    _sizes(what, *q.shape, Hkv, *(k_cache.shape[1:2] if k_cache is not None else ()))
     if (k_cache is None) != (v_cache is None) or (k_cache is None) != (slots is None):
         raise RuntimeError(f"{what}: give k_cache, v_cache and slots together")
     given = [t for t in (positions, inv_freq, q_weight, k_weight, k_cache, v_cache, slots) if t is not None]
@@ -1182,8 +1191,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """Log probabilities of given tokens, the entropy and the ``top_k`` most probable tokens of
     every row of logits, in one pass over them.
 
-    logits  [..., V] bf16, fp16 or fp32; rows of any alignment, up to three dimensions in any
-            strides (a shifted view of a text's logits is read in place)
+    logits  [..., V] bf16, fp16 or fp32, V at most 2^20 - 8; rows of any alignment, up to three
+            dimensions in any strides (a shifted view of a text's logits is read in place)
     tokens  [...] or [..., M] ids of each row (int64; other ints converted), or None
     top_k   at most 32
 
@@ -1198,6 +1207,7 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
             return TokenLogprobs(*done)
     if logits.dim() < 1 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise RuntimeError(f"{what}: logits [..., V] in bf16, fp16 or fp32 expected")
+    _sizes(what, *logits.shape, *(tokens.shape[-1:] if tokens is not None else ()))
     dev = _require_gpu(logits, *([tokens] if tokens is not None else []))
     _inference(what, logits, tokens)
     lead, V = logits.shape[:-1], logits.shape[-1]

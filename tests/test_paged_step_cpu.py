@@ -108,6 +108,33 @@ def test_cpu_tensors_are_refused():
         ops.token_logprobs(torch.zeros(2, 8))
 
 
+def test_sizes_past_32_bits_are_refused():
+    """The descriptors' fields would wrap them: 2^32 + 16 is no page size of 16."""
+    i, table, far = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32), 2 ** 32 + 16
+    for kw in (dict(page_size=far, width=1), dict(page_size=16, width=far), dict(page_size=16, rows=far),
+               dict(page_size=16, width=2 ** 30)):
+        with pytest.raises(RuntimeError, match="too large"):
+            ops.assign_pages(i, i, table, i, i[:1], **kw)
+    for args in ((table, i, far), (i[:1, None].expand(2, far), i, 16), (table, i[:1].expand(far), 16)):
+        with pytest.raises(RuntimeError, match="too large"):
+            ops.release_pages(i, i, args[0], args[1], i[:1], args[2])
+    f, one = torch.ones(4), torch.zeros(1, 1, 1, 8)
+    for shape in ((far, 1, 1, 8), (1, far, 1, 8)):
+        x = one.expand(shape)
+        with pytest.raises(RuntimeError, match="too large"):
+            ops.norm_rope_kv_write(x, x, x, i[:1].expand(shape[:2]), f)
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.norm_rope_kv_write(one.expand(1, 1, far, 8), one, one, i[:1, None], f)
+    pool = one.expand(1, far, 1, 8)
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.norm_rope_kv_write(one, one, one, i[:1, None], f, k_cache=pool, v_cache=pool, slots=i[:1, None])
+    for shape in ((far,), (2, far), (far, 2), (far, 2, 2)):
+        with pytest.raises(RuntimeError, match="too large"):
+            ops.token_logprobs(torch.zeros(1).expand(shape))
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.token_logprobs(torch.zeros(2, 8), i[:1].expand(2, far))
+
+
 @pytest.fixture(scope="module")
 def lib():
     if not _ffi.LIB_PATH.exists():
