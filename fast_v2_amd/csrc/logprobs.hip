@@ -42,6 +42,7 @@ constexpr int kStep = 2048 * kWaves;      // logits of a workgroup's step
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kCandidates = 1024;
 constexpr int kMaxTop = 32;
+constexpr int kMaxRows = (1 << 24) - 1;   // a launch has fewer than 2^32 threads, a row kThreads
 
 struct ScoreArgs {
   const void* logits;
@@ -571,7 +572,7 @@ int check_sizes(const char* what, int vocab, int64_t rows, int dtype) {
   FDLLM_CHECK_ARG(dtype == FDLLM_DTYPE_BF16 || dtype == FDLLM_DTYPE_F16 || dtype == FDLLM_DTYPE_F32,
                   "%s: dtype %d unsupported", what, dtype);
   FDLLM_CHECK_ARG(vocab > 0 && vocab <= kMaxVocab - 8, "%s: vocab %d (1 to %d)", what, vocab, kMaxVocab - 8);
-  FDLLM_CHECK_ARG(rows >= 0 && rows <= 0x7fffffff, "%s: bad row count", what);
+  FDLLM_CHECK_ARG(rows >= 0 && rows <= kMaxRows, "%s: %lld rows (0 to %d)", what, static_cast<long long>(rows), kMaxRows);
   return FDLLM_OK;
 }
 
@@ -602,7 +603,6 @@ extern "C" int fdllm_token_logprobs(const void* logits, int64_t stride_b, int64_
   FDLLM_CHECK_ARG(logits && entropy && (given == 0 || (tokens && logprobs)) && (top == 0 || (top_logprobs && top_tokens)),
                   "%s: null pointer", what);
   const Cut c = cut(vocab, rows, dtype);
-  FDLLM_CHECK_ARG(rows * c.splits <= 0x7fffffff, "%s: too many rows", what);
   if (c.bytes > 0 && (workspace == nullptr || workspace_bytes < c.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)) {
     set_last_error("%s: workspace of %zu bytes required (got %zu)", what, c.bytes, workspace_bytes);
     return FDLLM_ERR_WORKSPACE;

@@ -111,6 +111,7 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kTokenPerWave = 2048;
 constexpr int kResident = 2048;
 constexpr int kAhead = 2;  // a wave's steps in flight
+constexpr int kMaxTokens = (1 << 25) - 1;  // a launch has fewer than 2^32 threads, a token 64, and workgroups are whole
 
 // Sum over groups of L consecutive lanes.
 template <int L>
@@ -359,7 +360,7 @@ extern "C" int fdllm_norm_rope_kv_write(const fdllm_norm_rope_kv_desc* desc, voi
                   "%s: bad sizes", what);
   const int64_t tokens = static_cast<int64_t>(d.batch) * d.seq_len;
   if (tokens == 0) return FDLLM_OK;
-  FDLLM_CHECK_ARG(tokens <= 0x7fffffff, "%s: too many tokens", what);
+  FDLLM_CHECK_ARG(tokens <= kMaxTokens, "%s: %lld tokens (at most %d)", what, static_cast<long long>(tokens), kMaxTokens);
   FDLLM_CHECK_ARG(d.q && d.k && d.v && d.q_out && (d.rotary_dim == 0 || (d.positions && d.inv_freq)),
                   "%s: null pointer", what);
   FDLLM_CHECK_ARG((d.k_cache != nullptr) == (d.v_cache != nullptr) && (d.k_cache != nullptr) == (d.slots != nullptr),

@@ -1084,7 +1084,7 @@ def norm_rope_kv_write(
     into a page pool, in one kernel.
 
     q          [B, S, Hq, D], k / v [B, S, Hkv, D] bf16, fp16 or fp32 (a packed token list is
-               B = 1); D a multiple of 8, at most 256
+               B = 1), fewer than 2^25 tokens; D a multiple of 8, at most 256
     positions  [B, S] of the tokens (int32; other ints converted)
     inv_freq   [R / 2] fp32, R even, at most D: dimensions from R on are not rotated
                (``rope_frequencies`` makes it; rope_scale multiplies cos and sin)
@@ -1191,8 +1191,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     """Log probabilities of given tokens, the entropy and the ``top_k`` most probable tokens of
     every row of logits, in one pass over them.
 
-    logits  [..., V] bf16, fp16 or fp32, V at most 2^20 - 8; rows of any alignment, up to three
-            dimensions in any strides (a shifted view of a text's logits is read in place)
+    logits  [..., V] bf16, fp16 or fp32, V at most 2^20 - 8, fewer than 2^24 rows, of any alignment,
+            up to three dimensions in any strides (a shifted view of a text's logits is read in place)
     tokens  [...] or [..., M] ids of each row (int64; other ints converted), or None
     top_k   at most 32
 

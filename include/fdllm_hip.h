@@ -554,8 +554,8 @@ int fdllm_release_pages(const fdllm_page_pool* pool, const int32_t* keep_lens, v
  *   k_cache / v_cache / slots (all NULL) no pool is written and v is not read.
  *
  * positions, slots: [batch, seq_len] contiguous, int32 and int64. head_dim is a multiple of 8,
- * at most 256; rotary_dim even, at most head_dim. Rows and strides are multiples of 16 bytes.
- * q_out is contiguous. weight_dtype: the heads' dtype, or FDLLM_DTYPE_F32. No output may
+ * at most 256; rotary_dim even, at most head_dim; batch * seq_len below 2^25. Rows and strides are
+ * multiples of 16 bytes. q_out is contiguous. weight_dtype: the heads' dtype, or FDLLM_DTYPE_F32. No output may
  * overlap an input.
  *
  * Replaces, for paged caches: _apply_rotary_pos_emb + write_scratch_compiled
@@ -604,7 +604,7 @@ int fdllm_norm_rope_kv_write(const fdllm_norm_rope_kv_desc* desc, void* stream);
  *
  * `workspace` (fdllm_token_logprobs_workspace_size bytes, 0 for many rows; 16-byte aligned)
  * needs no initialisation; calls that may overlap in time need separate ones. One kernel, or two
- * where workgroups share a row. vocab is at most 2^20 - 8.
+ * where workgroups share a row. vocab is at most 2^20 - 8, and there are fewer than 2^24 rows.
  *
  * No counterpart in the reference, whose sampling takes the probability of the greedy token
  * (modeling.py:2263-2270); for scoring given texts.

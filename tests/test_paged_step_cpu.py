@@ -209,6 +209,22 @@ def test_c_abi_refuses_bad_scores(lib):
     assert call(batch=0) == 0
 
 
+def test_c_abi_refuses_more_than_a_launch_holds(lib):
+    """A launch has fewer than 2^32 threads: 64 a token, 256 a row."""
+    bad, size = _ffi.FDLLM_ERR_INVALID_ARGUMENT, ctypes.c_size_t(0)
+    d = _ffi.NormRopeKVDesc()
+    d.q = d.k = d.v = d.q_out = d.positions = d.inv_freq = 64
+    d.num_q_heads, d.num_kv_heads, d.head_dim, d.rotary_dim = 1, 1, 8, 8
+    d.dtype = d.weight_dtype = _ffi.DTYPE_BF16
+    for d.batch, d.seq_len in ((1 << 13, 1 << 13), (1, 1 << 26)):
+        assert lib.fdllm_norm_rope_kv_write(ctypes.byref(d), None) == bad
+        assert b"tokens" in lib.fdllm_last_error()
+    assert lib.fdllm_token_logprobs_workspace_size(8, 1 << 24, _ffi.DTYPE_BF16, ctypes.byref(size)) == bad
+    assert lib.fdllm_token_logprobs_workspace_size(8, (1 << 24) - 1, _ffi.DTYPE_BF16, ctypes.byref(size)) == 0
+    assert lib.fdllm_token_logprobs(64, 8, 8, 1 << 12, 1 << 12, 8, None, 0, 0, None, 64, None, None, _ffi.DTYPE_BF16, None,
+                                    0, None) == bad
+
+
 @pytest.mark.parametrize("struct,mirror", [("fdllm_page_pool", _ffi.PagePool),
                                            ("fdllm_norm_rope_kv_desc", _ffi.NormRopeKVDesc)])
 def test_descriptors_match_the_c_compiler(tmp_path, struct, mirror):
