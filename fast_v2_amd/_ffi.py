@@ -201,7 +201,7 @@ SIGNATURES = {
     "fdllm_assign_pages": (_c_int, [
         ctypes.POINTER(PagePool), _c_vp, _c_int, _c_int,  # pool, new_lens, width, rows
         _c_vp, _c_vp, _c_vp, _c_vp,                       # slots, positions, sequences, row_starts
-        _c_vp, _c_vp, _c_vp, _c_vp,                       # starts, seqlens, granted, stream
+        _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,                # starts, seqlens, granted, scratch, stream
     ]),
     "fdllm_release_pages": (_c_int, [ctypes.POINTER(PagePool), _c_vp, _c_vp]),  # pool, keep_lens, stream
     "fdllm_norm_rope_kv_write": (_c_int, [ctypes.POINTER(NormRopeKVDesc), _c_vp]),

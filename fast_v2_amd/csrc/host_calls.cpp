@@ -596,13 +596,14 @@ PyObject* assign(PyObject* const* a, Py_ssize_t n) {
   plain(n_rows <= INT32_MAX);
   Carve all;
   const int64_t at[] = {all.add(n_rows, 8), all.add(n_rows, 4), all.add(B, 4), all.add(B, 4), all.add(B, 4),
-                        all.add(width ? 0 : rows, 4), all.add(width ? 0 : B + 1, 4)};
+                        all.add(width ? 0 : rows, 4), all.add(width ? 0 : B + 1, 4),
+                        all.add(B, 4)};
   all.allocate(ask);
   const int64_t grid[] = {B, width};
   const at::IntArrayRef shape = width ? at::IntArrayRef(grid) : at::IntArrayRef(rows);
   Tensor slots = all.view(at[0], shape, at::kLong), positions = all.view(at[1], shape, at::kInt),
          starts = all.view(at[2], {B}, at::kInt), seqlens = all.view(at[3], {B}, at::kInt),
-         granted = all.view(at[4], {B}, at::kInt), sequences, row_starts;
+         granted = all.view(at[4], {B}, at::kInt), scratch = all.view(at[7], {B}, at::kInt), sequences, row_starts;
   if (!width) {
     sequences = all.view(at[5], {rows}, at::kInt);
     row_starts = all.view(at[6], {B + 1}, at::kInt);
@@ -611,7 +612,7 @@ PyObject* assign(PyObject* const* a, Py_ssize_t n) {
   const Stream s(ask);
   check(launch([&] { return api.assign(&p, ints(ask), static_cast<int>(width), static_cast<int>(rows),
                    static_cast<int64_t*>(slots.data_ptr()), ints(positions), ints(sequences), ints(row_starts),
-                   ints(starts), ints(seqlens), ints(granted), s.ptr); }),
+                   ints(starts), ints(seqlens), ints(granted), ints(scratch), s.ptr); }),
         "fdllm_assign_pages");
   return pack({&slots, &positions, &starts, &seqlens, &granted, &sequences, &row_starts});
 }

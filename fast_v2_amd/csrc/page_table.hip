@@ -8,14 +8,15 @@
 // d_b - 1), which is free_pages[free_count - 1 - i]. Rows of a packed token list begin at the
 // running sum of n. Both sums are one scan over the requests in one workgroup (saturating
 // 32-bit sums of non-negative numbers, which stay associative: what does not fit saturates
-// above every capacity). Because c is monotone, the requests that got pages are a prefix of
-// those that asked, so the request of page i is the first one with c_b > i: a binary search in
-// LDS, which spreads the pages of one long prompt over all threads as evenly as one page each
-// of many requests.
+// above every capacity). A new page's first row is a granted one, so the row that it begins with
+// enters it into the table, and the rows' threads take page ids from the free list by themselves. A
+// packed row's request, and of a page that goes back, is found by a binary search of the running sums
+// in LDS: long prompts are spread over all threads as evenly as single tokens.
 //
 // What bounds it: latency. The bytes of the largest call take 0.2 us; the calls are chains
-// of dependent memory round trips (arguments, lengths, free list or table, stores) and the scans' barriers:
-// 16 x 8 rows 3.5 us and 2.4 us to release them, 2048 x 32 rows (4096 pages) 8.5 + 2.6 and 4.7.
+// of dependent memory round trips (arguments, lengths, table or free list, stores) and the scans' barriers:
+// 16 x 8 rows 2.9 us and 2.4 us to release them, 2048 x 32 rows (4096 pages) 3.7 + 3.3 and 6.0. With the
+// pages searched and entered by the plan's workgroup the latter's first took 8.5.
 #include "fdllm_common.h"
 
 namespace fdllm {
@@ -24,7 +25,8 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxRequests = 8192;
 // Rows up to which the plan's workgroup makes them too. us, one kernel / two (assign and release): 16 x 8
-// rows 5.9 / 7.3, 256 x 16 8.4 / 9.3, 256 x 32 11.0 / 10.1, 1024 x 16 15.2 / 10.7, 2048 x 32 42 / 15.3.
+// rows 5.7 / 6.9, 256 x 16 7.8 / 8.3, 256 x 32 9.9 / 8.3, 1024 x 16 14.8 / 9.1; packed, 300 requests and
+// 4096 rows 9.1 / 10.1, 16 and 8192 11.8 / 9.9.
 constexpr int kOneKernelRows = 4096;
 
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
@@ -62,7 +64,7 @@ __device__ __forceinline__ int first_above(const uint32_t* upto, uint32_t i) {
   return at + (upto[at] <= i ? 1 : 0);
 }
 
-// Pages of a thread at a time: many requests need them (2048 x 32 rows 17.7 us with one, 15.3 with four), few
+// Pages of a thread's release at a time: many requests need them (2048 x 32 rows 17.7 us with one, 15.3 with four), few
 // are quicker in little code (16 x 8 rows 6.0 and 6.8).
 template <int ITEMS>
 constexpr int side() {
@@ -80,10 +82,30 @@ struct AssignArgs {
   int32_t* starts;
   int32_t* seqlens;
   int32_t* granted;
+  int32_t* list_at;  // of the rows' kernel: a request's page j, if it is new, is the free list's entry list_at - j
 };
 
-// Row r: the request's t-th asked token (b < 0: none), at position pos.
-__device__ __forceinline__ void put_row(const AssignArgs& a, int r, int b, int64_t pos, int64_t slot) {
+// Row r: the request's t-th asked token (b < 0: none), from its length before the step. A page in hand
+// comes from the table, a new one from the free list; its first row enters it.
+__device__ __forceinline__ void put_row(const AssignArgs& a, int r, int b, int t, uint32_t len, bool ok, int32_t list_at) {
+  const fdllm_page_pool& p = a.pool;
+  const uint32_t mask = (1u << a.shift) - 1;
+  int64_t pos = 0, slot = -1;
+  if (b >= 0) {
+    pos = static_cast<int64_t>(len) + t;
+    if (ok) {
+      const uint32_t j = static_cast<uint32_t>(pos >> a.shift), off = static_cast<uint32_t>(pos) & mask;
+      int32_t* const entry = p.page_table + b * p.table_stride + j;
+      int32_t page;
+      if (j < (len + mask) >> a.shift) {
+        page = *entry;
+      } else {
+        page = p.free_pages[list_at - static_cast<int32_t>(j)];
+        if (off == 0) *entry = page;
+      }
+      slot = (static_cast<int64_t>(page) << a.shift) + off;
+    }
+  }
   a.slots[r] = slot;
   a.positions[r] = static_cast<int32_t>(pos);
   if (a.sequences) a.sequences[r] = b;
@@ -94,17 +116,13 @@ __device__ __forceinline__ void put_row(const AssignArgs& a, int r, int b, int64
 template <int ITEMS, bool ROWS>
 __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignArgs a, int n_rows) {
   __shared__ uint32_t s_wave[2][kPlanThreads / 64];
-  __shared__ uint32_t s_upto[kPlanThreads * ITEMS];  // running sum of the needs
-  __shared__ int32_t s_at[kPlanThreads * ITEMS];     // table column of page i: s_at + i
+  __shared__ int32_t s_at[ROWS ? kPlanThreads * ITEMS : 1];     // list_at
   __shared__ uint32_t s_end[ROWS ? kPlanThreads * ITEMS : 1];  // running sum of the asked tokens
   __shared__ uint32_t s_len[ROWS ? kPlanThreads * ITEMS : 1];  // length, the top bit: granted
   __shared__ uint32_t s_new[ROWS ? kPlanThreads * ITEMS : 1];
-  __shared__ uint32_t s_taken;
-  constexpr int kSide = side<ITEMS>();
   const fdllm_page_pool& p = a.pool;
   const int tid = threadIdx.x;
   const uint32_t mask = (1u << a.shift) - 1;
-  if (tid == 0) s_taken = 0;
   const int count = *p.free_count;
   uint32_t n[ITEMS], len[ITEMS], need[ITEMS], have[ITEMS];
   int32_t old[ITEMS];
@@ -137,17 +155,17 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
     sum_need = add_sat(sum_need, need[k]);
   }
   uint32_t c = block_scan(sum_need, s_wave[1]).before;
-  uint32_t taken = 0;
+  uint32_t taken = c;
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int b = tid * ITEMS + k;
-    s_at[b] = static_cast<int32_t>(have[k] - c);
+    const int32_t list_at = static_cast<int32_t>(avail - 1 + have[k] - c);
     c = add_sat(c, need[k]);
-    s_upto[b] = c;
+    if (c <= avail) taken = c;
     const bool ok = asks[k] && (need[k] == 0 || c <= avail);
-    if (ok) taken = max(taken, need[k] ? c : 0);
     const uint32_t got = ok ? n[k] : 0;
     if (ROWS) {
+      s_at[b] = list_at;
       s_len[b] = len[k] | (ok ? 0x80000000u : 0);
       s_new[b] = n[k];
     }
@@ -155,28 +173,14 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
       a.starts[b] = static_cast<int32_t>(len[k]);
       a.seqlens[b] = static_cast<int32_t>(len[k] + got);
       a.granted[b] = static_cast<int32_t>(got);
+      if (!ROWS) a.list_at[b] = list_at;
       if (got != 0 || old[k] < 0) p.lens[b] = static_cast<int32_t>(len[k] + got);
     }
   }
-  if (taken) atomicMax(&s_taken, taken);
-  __syncthreads();
-  taken = s_taken;
-  if (tid == 0) *p.free_count = static_cast<int32_t>(avail - taken);
-  for (uint32_t i0 = tid; i0 < taken; i0 += kSide * kPlanThreads) {
-    int b[kSide], page[kSide];
-#pragma unroll
-    for (int k = 0; k < kSide; ++k) {
-      const uint32_t i = min(i0 + k * kPlanThreads, taken - 1);  // the last one may be written twice
-      b[k] = first_above<kPlanThreads * ITEMS>(s_upto, i);
-      page[k] = p.free_pages[avail - 1 - i];
-    }
-#pragma unroll
-    for (int k = 0; k < kSide; ++k) {
-      const uint32_t i = min(i0 + k * kPlanThreads, taken - 1);
-      p.page_table[b[k] * p.table_stride + static_cast<int32_t>(s_at[b[k]] + i)] = page[k];
-    }
-  }
+  // by the one thread behind whose requests the pages have run out, or the last
+  if (taken <= avail && (c > avail || tid == kPlanThreads - 1)) *p.free_count = static_cast<int32_t>(avail - taken);
   if constexpr (ROWS) {
+    __syncthreads();
 #pragma unroll 1
     for (int r = tid; r < n_rows; r += kPlanThreads) {
       int b, t;
@@ -189,19 +193,8 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
         t = b < p.requests ? r - static_cast<int>(s_end[b] - s_new[b]) : 0;  // an end past r and a begin at most r: no saturation
         if (b >= p.requests) b = -1;
       }
-      int64_t pos = 0, slot = -1;
-      if (b >= 0) {
-        const uint32_t l = s_len[b];
-        pos = static_cast<int64_t>(l & 0x7fffffffu) + t;
-        if (l >> 31) {
-          // a page in hand from the table, a new one from the free list: this kernel's stores need not be read back
-          const uint32_t j = static_cast<uint32_t>(pos >> a.shift);
-          const int32_t page = j < (((l & 0x7fffffffu) + mask) >> a.shift) ? p.page_table[b * p.table_stride + j]
-                                                                          : p.free_pages[avail - 1 - (j - s_at[b])];
-          slot = (static_cast<int64_t>(page) << a.shift) + (pos & mask);
-        }
-      }
-      put_row(a, r, b, pos, slot);
+      const uint32_t len = b >= 0 ? s_len[b] : 0;
+      put_row(a, r, b, t, len & 0x7fffffffu, len >> 31, b >= 0 ? s_at[b] : 0);
     }
   }
 }
@@ -229,14 +222,8 @@ __global__ __launch_bounds__(kRowsPerWg) void assign_rows_kernel(const AssignArg
     t = b < p.requests ? r - a.row_starts[b] : 0;
     if (b >= p.requests) b = -1;
   }
-  int64_t pos = 0, slot = -1;
-  if (b >= 0) {
-    pos = static_cast<int64_t>(a.starts[b]) + t;
-    if (a.granted[b] > 0)
-      slot = (static_cast<int64_t>(p.page_table[b * p.table_stride + (pos >> a.shift)]) << a.shift) +
-             (pos & ((1 << a.shift) - 1));
-  }
-  put_row(a, r, b, pos, slot);
+  if (b >= 0) put_row(a, r, b, t, static_cast<uint32_t>(a.starts[b]), a.granted[b] > 0, a.list_at[b]);
+  else put_row(a, r, -1, 0, 0, false, 0);
 }
 
 // keep_lens: pages behind the kept lengths go back, the last ones first.
@@ -314,7 +301,7 @@ int check_pool(const char* what, const fdllm_page_pool* p) {
 
 extern "C" int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* new_lens, int width, int rows,
                                   int64_t* slots, int32_t* positions, int32_t* sequences, int32_t* row_starts,
-                                  int32_t* starts, int32_t* seqlens, int32_t* granted, void* stream) {
+                                  int32_t* starts, int32_t* seqlens, int32_t* granted, int32_t* scratch, void* stream) {
   using namespace fdllm;
   const char* what = "fdllm_assign_pages";
   if (const int rc = check_pool(what, pool)) return rc;
@@ -322,7 +309,7 @@ extern "C" int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* ne
                   "%s: give the padded form's width or the packed form's rows", what);
   if (pool->requests == 0 && width > 0) return FDLLM_OK;
   FDLLM_CHECK_ARG(pool->requests > 0, "%s: a packed list without requests", what);
-  FDLLM_CHECK_ARG(new_lens && slots && positions && starts && seqlens && granted && (width > 0 || (sequences && row_starts)),
+  FDLLM_CHECK_ARG(new_lens && slots && positions && starts && seqlens && granted && scratch && (width > 0 || (sequences && row_starts)),
                   "%s: null pointer", what);
   AssignArgs a;
   a.pool = *pool;
@@ -337,6 +324,7 @@ extern "C" int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* ne
   a.starts = starts;
   a.seqlens = seqlens;
   a.granted = granted;
+  a.list_at = scratch;
   const int64_t all_rows = width > 0 ? static_cast<int64_t>(width) * pool->requests : rows;
   FDLLM_CHECK_ARG(all_rows <= 0x7fffffff - kRowsPerWg, "%s: too many rows", what);
   const int n_rows = static_cast<int>(all_rows);

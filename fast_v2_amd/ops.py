@@ -1000,7 +1000,7 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.T
     shape = (B, width) if width else (rows,)
     slots = torch.empty(shape, dtype=torch.int64, device=dev)
     positions = torch.empty(shape, dtype=torch.int32, device=dev)
-    starts, seqlens, granted = (torch.empty(B, dtype=torch.int32, device=dev) for _ in range(3))
+    starts, seqlens, granted, scratch = (torch.empty(B, dtype=torch.int32, device=dev) for _ in range(4))
     sequences = row_starts = None
     if not width:
         sequences = torch.empty(rows, dtype=torch.int32, device=dev)
@@ -1009,7 +1009,7 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.T
         rc = _ffi.lib().fdllm_assign_pages(
             ctypes.byref(p), new_lens.data_ptr(), int(width), int(rows), slots.data_ptr(), positions.data_ptr(),
             _ptr(sequences), _ptr(row_starts), starts.data_ptr(), seqlens.data_ptr(), granted.data_ptr(),
-            _ffi.stream_ptr(dev))
+            scratch.data_ptr(), _ffi.stream_ptr(dev))
     _ffi.check(rc, "fdllm_assign_pages")
     return PageRows(slots, positions, starts, seqlens, granted, sequences, row_starts)
 

@@ -515,7 +515,7 @@ int fdllm_unmask_step_ws(const void* logits, int64_t logits_stride_b, int64_t lo
  *   or -1, row_starts[requests + 1] the rows' prefix sums (at most INT32_MAX). Per request:
  *   starts (lens before), seqlens (lens after), granted.
  *   sequences and row_starts are NULL in the padded form. Table columns of pages that were not
- *   handed out keep what they hold.
+ *   handed out keep what they hold. scratch: [requests], of any content.
  *
  * fdllm_release_pages: lens[b] becomes min(lens[b], max(keep_lens[b], 0)); pages behind it go
  *   back to the free list, in the reverse of the order in which fdllm_assign_pages hands them
@@ -535,7 +535,7 @@ typedef struct fdllm_page_pool {
 
 int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* new_lens, int width, int rows, int64_t* slots,
                        int32_t* positions, int32_t* sequences, int32_t* row_starts, int32_t* starts,
-                       int32_t* seqlens, int32_t* granted, void* stream);
+                       int32_t* seqlens, int32_t* granted, int32_t* scratch, void* stream);
 int fdllm_release_pages(const fdllm_page_pool* pool, const int32_t* keep_lens, void* stream);
 
 /* -------------------------------------------------------------------------

@@ -150,7 +150,7 @@ def test_c_abi_refuses_bad_pools(lib):
         return p
 
     def assign(p, width=1, rows=0, seq=None):
-        return lib.fdllm_assign_pages(ctypes.byref(p) if p else None, 16, width, rows, 16, 16, seq, seq, 16, 16, 16, None)
+        return lib.fdllm_assign_pages(ctypes.byref(p) if p else None, 16, width, rows, 16, 16, seq, seq, 16, 16, 16, 16, None)
     bad = _ffi.FDLLM_ERR_INVALID_ARGUMENT
     for kw in (dict(requests=-1), dict(requests=8193), dict(page_size=0), dict(page_size=24), dict(max_pages=-1),
                dict(num_free=-1), dict(table_stride=3), dict(lens=None), dict(free_count=None), dict(page_table=None),
