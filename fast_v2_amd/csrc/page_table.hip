@@ -31,27 +31,46 @@ constexpr int kOneKernelRows = 4096;
 
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
-// The sum over the threads before this one, and over all.
-struct Scan {
-  uint32_t before, all;
-};
-__device__ __forceinline__ Scan block_scan(uint32_t x, uint32_t* s_wave) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// A thread's k-th request: neighbouring lanes take neighbouring ones, so that loads and stores are whole lines.
+template <int ITEMS>
+__device__ __forceinline__ int request_of(int k) {
+  return (threadIdx.x & ~63u) * ITEMS + k * 64 + (threadIdx.x & 63u);
+}
+
+// x from another lane of the wave; 0 where there is none, or outside of the rows (of 16 lanes) in ROWS
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_up(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, ROWS, 0xf, false));
+}
+
+// Per request the sum over those before it; returns the sum over all.
+template <int ITEMS>
+__device__ __forceinline__ uint32_t block_scan(const uint32_t (&x)[ITEMS], uint32_t (&before)[ITEMS], uint32_t* s_wave) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t of_wave = 0;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t up = __shfl_up(x, o, kWave);
-    if (lane >= o) x = add_sat(x, up);
+  for (int k = 0; k < ITEMS; ++k) {
+    uint32_t y = x[k];
+    y = add_sat(y, dpp_up<0x111, 0xf>(y));  // from 1, 2, 4 and 8 lanes below in a row
+    y = add_sat(y, dpp_up<0x112, 0xf>(y));
+    y = add_sat(y, dpp_up<0x114, 0xf>(y));
+    y = add_sat(y, dpp_up<0x118, 0xf>(y));
+    y = add_sat(y, dpp_up<0x142, 0xa>(y));  // a row's last lane to the next row: 0 to 1, 2 to 3
+    y = add_sat(y, dpp_up<0x143, 0xc>(y));  // lane 31 to rows 2 and 3
+    before[k] = add_sat(of_wave, dpp_up<0x138, 0xf>(y));  // from the lane below: saturated sums do not subtract
+    of_wave = add_sat(of_wave, __builtin_amdgcn_readlane(y, 63));
   }
-  if (lane == 63) s_wave[wave] = x;
-  const uint32_t up = __shfl_up(x, 1, kWave);  // saturated sums do not subtract
+  if ((threadIdx.x & 63) == 0) s_wave[wave] = of_wave;
   __syncthreads();
-  Scan r{0, 0};
+  uint32_t lower = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w == wave) r.before = add_sat(r.all, lane != 0 ? up : 0);
-    r.all = add_sat(r.all, s_wave[w]);
+    if (w == wave) lower = all;
+    all = add_sat(all, s_wave[w]);
   }
-  return r;
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) before[k] = add_sat(lower, before[k]);
+  return all;
 }
 
 // First b with upto[b] > i, of N (a power of two) entries; N where there is none. Without branches, so
@@ -112,7 +131,7 @@ __device__ __forceinline__ void put_row(const AssignArgs& a, int r, int b, int t
 }
 
 // The requests' part, and in the form of one kernel (ROWS) the rows': one workgroup, ITEMS
-// consecutive requests per thread.
+// requests per thread.
 template <int ITEMS, bool ROWS>
 __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignArgs a, int n_rows) {
   __shared__ uint32_t s_wave[2][kPlanThreads / 64];
@@ -124,44 +143,44 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
   const int tid = threadIdx.x;
   const uint32_t mask = (1u << a.shift) - 1;
   const int count = *p.free_count;
-  uint32_t n[ITEMS], len[ITEMS], need[ITEMS], have[ITEMS];
+  uint32_t n[ITEMS], len[ITEMS], need[ITEMS], have[ITEMS], at[ITEMS], before[ITEMS];
   int32_t old[ITEMS];
   bool asks[ITEMS];
-  uint32_t sum_n = 0, sum_need = 0;
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int b = tid * ITEMS + k;
+    const int b = request_of<ITEMS>(k);
     n[k] = b < p.requests ? max(a.new_lens[b], 0) : 0;
     old[k] = b < p.requests ? p.lens[b] : 0;
     len[k] = max(old[k], 0);
-    sum_n = add_sat(sum_n, n[k]);
   }
   // rows first (their sum does not depend on what is granted), then the needs of those that fit
-  uint32_t at = a.width > 0 ? 0 : block_scan(sum_n, s_wave[0]).before;
+  if (a.width == 0) block_scan<ITEMS>(n, at, s_wave[0]);
   const uint32_t avail = static_cast<uint32_t>(min(max(count, 0), p.num_free));
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int b = tid * ITEMS + k;
-    if (a.row_starts && b < p.requests) a.row_starts[b] = static_cast<int32_t>(min(at, 0x7fffffffu));
-    at = add_sat(at, n[k]);
-    if (a.row_starts && b == p.requests - 1) a.row_starts[p.requests] = static_cast<int32_t>(min(at, 0x7fffffffu));
-    if (ROWS) s_end[b] = at;
+    const int b = request_of<ITEMS>(k);
+    const uint32_t end = a.width > 0 ? 0 : add_sat(at[k], n[k]);
+    if (a.row_starts && b < p.requests) {
+      a.row_starts[b + 1] = static_cast<int32_t>(min(end, 0x7fffffffu));
+      if (b == 0) a.row_starts[0] = 0;
+    }
+    if (ROWS) s_end[b] = end;
     // lengths are below 2^31, so their sum fits 32 unsigned bits
     const uint32_t total = (len[k] + n[k] + mask) >> a.shift;
     have[k] = (len[k] + mask) >> a.shift;
     asks[k] = n[k] > 0 && len[k] + n[k] <= 0x7fffffffu && total <= static_cast<uint32_t>(p.max_pages) &&
-              (a.width > 0 ? n[k] <= static_cast<uint32_t>(a.width) : at <= static_cast<uint32_t>(a.rows));
+              (a.width > 0 ? n[k] <= static_cast<uint32_t>(a.width) : end <= static_cast<uint32_t>(a.rows));
     need[k] = asks[k] ? total - have[k] : 0;
-    sum_need = add_sat(sum_need, need[k]);
   }
-  uint32_t c = block_scan(sum_need, s_wave[1]).before;
-  uint32_t taken = c;
+  block_scan<ITEMS>(need, before, s_wave[1]);
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int b = tid * ITEMS + k;
-    const int32_t list_at = static_cast<int32_t>(avail - 1 + have[k] - c);
-    c = add_sat(c, need[k]);
-    if (c <= avail) taken = c;
+    const int b = request_of<ITEMS>(k);
+    const int32_t list_at = static_cast<int32_t>(avail - 1 + have[k] - before[k]);
+    const uint32_t c = add_sat(before[k], need[k]);
+    // by the one request at which the pages run out, or the last
+    if (before[k] <= avail && (c > avail || b == kPlanThreads * ITEMS - 1))
+      *p.free_count = static_cast<int32_t>(avail - (c > avail ? before[k] : c));
     const bool ok = asks[k] && (need[k] == 0 || c <= avail);
     const uint32_t got = ok ? n[k] : 0;
     if (ROWS) {
@@ -177,8 +196,6 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
       if (got != 0 || old[k] < 0) p.lens[b] = static_cast<int32_t>(len[k] + got);
     }
   }
-  // by the one thread behind whose requests the pages have run out, or the last
-  if (taken <= avail && (c > avail || tid == kPlanThreads - 1)) *p.free_count = static_cast<int32_t>(avail - taken);
   if constexpr (ROWS) {
     __syncthreads();
 #pragma unroll 1
@@ -243,10 +260,10 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const ReleaseArgs
   const int tid = threadIdx.x;
   const uint32_t count = static_cast<uint32_t>(min(max(*p.free_count, 0), p.num_free));
   const uint32_t mask = (1u << a.shift) - 1;
-  uint32_t kept[ITEMS], back[ITEMS], sum = 0;
+  uint32_t kept[ITEMS], back[ITEMS], before[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    const int b = tid * ITEMS + k;
+    const int b = request_of<ITEMS>(k);
     kept[k] = back[k] = 0;
     if (b < p.requests) {
       const uint32_t len = max(p.lens[b], 0);
@@ -256,16 +273,12 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const ReleaseArgs
       back[k] = min((len + mask) >> a.shift, most) - kept[k];
       p.lens[b] = static_cast<int32_t>(keep);
     }
-    sum = add_sat(sum, back[k]);
   }
-  const Scan scan = block_scan(sum, s_wave);
-  uint32_t c = scan.before;
-  const uint32_t n = min(scan.all, static_cast<uint32_t>(p.num_free) - count);
+  const uint32_t n = min(block_scan<ITEMS>(back, before, s_wave), static_cast<uint32_t>(p.num_free) - count);
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
-    s_at[tid * ITEMS + k] = static_cast<int32_t>(kept[k] - c);
-    c = add_sat(c, back[k]);
-    s_upto[tid * ITEMS + k] = c;
+    s_at[request_of<ITEMS>(k)] = static_cast<int32_t>(kept[k] - before[k]);
+    s_upto[request_of<ITEMS>(k)] = add_sat(before[k], back[k]);
   }
   __syncthreads();
   for (uint32_t i0 = tid; i0 < n; i0 += kSide * kPlanThreads) {
