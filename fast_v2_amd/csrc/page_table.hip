@@ -15,18 +15,23 @@
 //
 // What bounds it: latency. The bytes of the largest call take 0.2 us; the calls are chains
 // of dependent memory round trips (arguments, lengths, table or free list, stores) and the scans' barriers:
-// 16 x 8 rows 2.9 us and 2.4 us to release them, 2048 x 32 rows (4096 pages) 3.7 + 3.3 and 6.0. With the
-// pages searched and entered by the plan's workgroup the latter's first took 8.5.
+// 16 x 8 rows 2.3 us and 2.0 us to release them, 2048 x 32 rows (4096 pages) 2.8 + 3.5 and 5.4. With the
+// pages searched and entered by the plan's workgroup the plan took 8.5, and with scans that exchange through
+// LDS each scan 0.5 us more.
 #include "fdllm_common.h"
 
 namespace fdllm {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+// Threads where there are at most as many requests and, to assign, rows. us, 256 / 1024 (assign and
+// release): 16 x 8 rows 4.3 / 4.6, 64 x 8 4.9 / 4.6; to release up to 256 pages 0.15 less, 512 0.2 more, 4096 4.5
+// more (once a request, the others at every step).
+constexpr int kSmallThreads = 256;
 constexpr int kMaxRequests = 8192;
 // Rows up to which the plan's workgroup makes them too. us, one kernel / two (assign and release): 16 x 8
-// rows 5.7 / 6.9, 256 x 16 7.8 / 8.3, 256 x 32 9.9 / 8.3, 1024 x 16 14.8 / 9.1; packed, 300 requests and
-// 4096 rows 9.1 / 10.1, 16 and 8192 11.8 / 9.9.
+// rows 4.3 / 5.8, 256 x 16 6.5 / 7.0, 256 x 32 8.7 / 7.0, 1024 x 16 13.5 / 7.9; packed, 300 requests and
+// 4096 rows 7.4 / 8.5, 16 and 8192 10.1 / 8.0.
 constexpr int kOneKernelRows = 4096;
 
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
@@ -44,7 +49,7 @@ __device__ __forceinline__ uint32_t dpp_up(uint32_t x) {
 }
 
 // Per request the sum over those before it; returns the sum over all.
-template <int ITEMS>
+template <int T, int ITEMS>
 __device__ __forceinline__ uint32_t block_scan(const uint32_t (&x)[ITEMS], uint32_t (&before)[ITEMS], uint32_t* s_wave) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t of_wave = 0;
@@ -62,15 +67,17 @@ __device__ __forceinline__ uint32_t block_scan(const uint32_t (&x)[ITEMS], uint3
   }
   if ((threadIdx.x & 63) == 0) s_wave[wave] = of_wave;
   __syncthreads();
-  uint32_t lower = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w == wave) lower = all;
-    all = add_sat(all, s_wave[w]);
+  uint32_t y = s_wave[threadIdx.x & (T / 64 - 1)];
+  y = add_sat(y, dpp_up<0x111, 0xf>(y));
+  y = add_sat(y, dpp_up<0x112, 0xf>(y));
+  if constexpr (T > 256) {
+    y = add_sat(y, dpp_up<0x114, 0xf>(y));
+    y = add_sat(y, dpp_up<0x118, 0xf>(y));
   }
+  const uint32_t lower = wave != 0 ? __builtin_amdgcn_readlane(y, max(wave - 1, 0)) : 0;
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) before[k] = add_sat(lower, before[k]);
-  return all;
+  return __builtin_amdgcn_readlane(y, T / 64 - 1);
 }
 
 // First b with upto[b] > i, of N (a power of two) entries; N where there is none. Without branches, so
@@ -83,8 +90,8 @@ __device__ __forceinline__ int first_above(const uint32_t* upto, uint32_t i) {
   return at + (upto[at] <= i ? 1 : 0);
 }
 
-// Pages of a thread's release at a time: many requests need them (2048 x 32 rows 17.7 us with one, 15.3 with four), few
-// are quicker in little code (16 x 8 rows 6.0 and 6.8).
+// Pages of a thread's release at a time: many requests need them, few are quicker in little code, which is
+// loaded for every call (16 requests of 8 pages 0.3 us less with one than with four).
 template <int ITEMS>
 constexpr int side() {
   return ITEMS == 1 ? 1 : 4;
@@ -132,13 +139,13 @@ __device__ __forceinline__ void put_row(const AssignArgs& a, int r, int b, int t
 
 // The requests' part, and in the form of one kernel (ROWS) the rows': one workgroup, ITEMS
 // requests per thread.
-template <int ITEMS, bool ROWS>
-__global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignArgs a, int n_rows) {
-  __shared__ uint32_t s_wave[2][kPlanThreads / 64];
-  __shared__ int32_t s_at[ROWS ? kPlanThreads * ITEMS : 1];     // list_at
-  __shared__ uint32_t s_end[ROWS ? kPlanThreads * ITEMS : 1];  // running sum of the asked tokens
-  __shared__ uint32_t s_len[ROWS ? kPlanThreads * ITEMS : 1];  // length, the top bit: granted
-  __shared__ uint32_t s_new[ROWS ? kPlanThreads * ITEMS : 1];
+template <int T, int ITEMS, bool ROWS>
+__global__ __launch_bounds__(T) void assign_plan_kernel(const AssignArgs a, int n_rows) {
+  __shared__ uint32_t s_wave[2][T / 64];
+  __shared__ int32_t s_at[ROWS ? T * ITEMS : 1];     // list_at
+  __shared__ uint32_t s_end[ROWS ? T * ITEMS : 1];  // running sum of the asked tokens
+  __shared__ uint32_t s_len[ROWS ? T * ITEMS : 1];  // length, the top bit: granted
+  __shared__ uint32_t s_new[ROWS ? T * ITEMS : 1];
   const fdllm_page_pool& p = a.pool;
   const int tid = threadIdx.x;
   const uint32_t mask = (1u << a.shift) - 1;
@@ -154,7 +161,7 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
     len[k] = max(old[k], 0);
   }
   // rows first (their sum does not depend on what is granted), then the needs of those that fit
-  if (a.width == 0) block_scan<ITEMS>(n, at, s_wave[0]);
+  if (a.width == 0) block_scan<T, ITEMS>(n, at, s_wave[0]);
   const uint32_t avail = static_cast<uint32_t>(min(max(count, 0), p.num_free));
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
@@ -172,14 +179,14 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
               (a.width > 0 ? n[k] <= static_cast<uint32_t>(a.width) : end <= static_cast<uint32_t>(a.rows));
     need[k] = asks[k] ? total - have[k] : 0;
   }
-  block_scan<ITEMS>(need, before, s_wave[1]);
+  block_scan<T, ITEMS>(need, before, s_wave[1]);
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int b = request_of<ITEMS>(k);
     const int32_t list_at = static_cast<int32_t>(avail - 1 + have[k] - before[k]);
     const uint32_t c = add_sat(before[k], need[k]);
     // by the one request at which the pages run out, or the last
-    if (before[k] <= avail && (c > avail || b == kPlanThreads * ITEMS - 1))
+    if (before[k] <= avail && (c > avail || b == T * ITEMS - 1))
       *p.free_count = static_cast<int32_t>(avail - (c > avail ? before[k] : c));
     const bool ok = asks[k] && (need[k] == 0 || c <= avail);
     const uint32_t got = ok ? n[k] : 0;
@@ -199,14 +206,14 @@ __global__ __launch_bounds__(kPlanThreads) void assign_plan_kernel(const AssignA
   if constexpr (ROWS) {
     __syncthreads();
 #pragma unroll 1
-    for (int r = tid; r < n_rows; r += kPlanThreads) {
+    for (int r = tid; r < n_rows; r += T) {
       int b, t;
       if (a.width > 0) {
         b = static_cast<int>(static_cast<uint32_t>(r) / static_cast<uint32_t>(a.width));
         t = r - b * a.width;
         if (static_cast<uint32_t>(t) >= s_new[b]) b = -1;
       } else {
-        b = first_above<kPlanThreads * ITEMS>(s_end, static_cast<uint32_t>(r));
+        b = first_above<T * ITEMS>(s_end, static_cast<uint32_t>(r));
         t = b < p.requests ? r - static_cast<int>(s_end[b] - s_new[b]) : 0;  // an end past r and a begin at most r: no saturation
         if (b >= p.requests) b = -1;
       }
@@ -250,11 +257,11 @@ struct ReleaseArgs {
   int shift;
 };
 
-template <int ITEMS>
-__global__ __launch_bounds__(kPlanThreads) void release_kernel(const ReleaseArgs a) {
-  __shared__ uint32_t s_wave[kPlanThreads / 64];
-  __shared__ uint32_t s_upto[kPlanThreads * ITEMS];
-  __shared__ int32_t s_at[kPlanThreads * ITEMS];
+template <int T, int ITEMS>
+__global__ __launch_bounds__(T) void release_kernel(const ReleaseArgs a) {
+  __shared__ uint32_t s_wave[T / 64];
+  __shared__ uint32_t s_upto[T * ITEMS];
+  __shared__ int32_t s_at[T * ITEMS];
   constexpr int kSide = side<ITEMS>();
   const fdllm_page_pool& p = a.pool;
   const int tid = threadIdx.x;
@@ -274,23 +281,23 @@ __global__ __launch_bounds__(kPlanThreads) void release_kernel(const ReleaseArgs
       p.lens[b] = static_cast<int32_t>(keep);
     }
   }
-  const uint32_t n = min(block_scan<ITEMS>(back, before, s_wave), static_cast<uint32_t>(p.num_free) - count);
+  const uint32_t n = min(block_scan<T, ITEMS>(back, before, s_wave), static_cast<uint32_t>(p.num_free) - count);
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     s_at[request_of<ITEMS>(k)] = static_cast<int32_t>(kept[k] - before[k]);
     s_upto[request_of<ITEMS>(k)] = add_sat(before[k], back[k]);
   }
   __syncthreads();
-  for (uint32_t i0 = tid; i0 < n; i0 += kSide * kPlanThreads) {
+  for (uint32_t i0 = tid; i0 < n; i0 += kSide * T) {
     int page[kSide];
 #pragma unroll
     for (int k = 0; k < kSide; ++k) {
-      const uint32_t i = min(i0 + k * kPlanThreads, n - 1);  // the last one may be written twice
-      const int b = first_above<kPlanThreads * ITEMS>(s_upto, i);
+      const uint32_t i = min(i0 + k * T, n - 1);  // the last one may be written twice
+      const int b = first_above<T * ITEMS>(s_upto, i);
       page[k] = p.page_table[b * p.table_stride + static_cast<int32_t>(s_at[b] + i)];
     }
 #pragma unroll
-    for (int k = 0; k < kSide; ++k) p.free_pages[count + n - 1 - min(i0 + k * kPlanThreads, n - 1)] = page[k];
+    for (int k = 0; k < kSide; ++k) p.free_pages[count + n - 1 - min(i0 + k * T, n - 1)] = page[k];
   }
   if (tid == 0) *p.free_count = static_cast<int32_t>(count + n);
 }
@@ -342,15 +349,17 @@ extern "C" int fdllm_assign_pages(const fdllm_page_pool* pool, const int32_t* ne
   FDLLM_CHECK_ARG(all_rows <= 0x7fffffff - kRowsPerWg, "%s: too many rows", what);
   const int n_rows = static_cast<int>(all_rows);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int B = pool->requests, T = kPlanThreads;
+  const int B = pool->requests;
+  constexpr int T = kPlanThreads, S = kSmallThreads;
   if (B <= 2 * T && n_rows <= kOneKernelRows) {
-    if (B <= T) assign_plan_kernel<1, true><<<dim3(1), dim3(T), 0, s>>>(a, n_rows);
-    else assign_plan_kernel<2, true><<<dim3(1), dim3(T), 0, s>>>(a, n_rows);
+    if (B <= S && n_rows <= S) assign_plan_kernel<S, 1, true><<<dim3(1), dim3(S), 0, s>>>(a, n_rows);
+    else if (B <= T) assign_plan_kernel<T, 1, true><<<dim3(1), dim3(T), 0, s>>>(a, n_rows);
+    else assign_plan_kernel<T, 2, true><<<dim3(1), dim3(T), 0, s>>>(a, n_rows);
     FDLLM_RETURN_LAUNCH_STATUS(what);
   }
-  if (B <= T) assign_plan_kernel<1, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
-  else if (B <= 2 * T) assign_plan_kernel<2, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
-  else assign_plan_kernel<kMaxRequests / T, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
+  if (B <= T) assign_plan_kernel<T, 1, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
+  else if (B <= 2 * T) assign_plan_kernel<T, 2, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
+  else assign_plan_kernel<T, kMaxRequests / T, false><<<dim3(1), dim3(T), 0, s>>>(a, 0);
   const dim3 grid(static_cast<unsigned>((n_rows + kRowsPerWg - 1) / kRowsPerWg));
   if (width > 0 || B <= T) assign_rows_kernel<T><<<grid, dim3(kRowsPerWg), 0, s>>>(a, n_rows);
   else assign_rows_kernel<kMaxRequests><<<grid, dim3(kRowsPerWg), 0, s>>>(a, n_rows);
@@ -365,8 +374,11 @@ extern "C" int fdllm_release_pages(const fdllm_page_pool* pool, const int32_t* k
   FDLLM_CHECK_ARG(keep_lens != nullptr, "%s: null pointer", what);
   ReleaseArgs a{*pool, keep_lens, __builtin_ctz(static_cast<unsigned>(pool->page_size))};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (pool->requests <= kPlanThreads) release_kernel<1><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
-  else if (pool->requests <= 2 * kPlanThreads) release_kernel<2><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
-  else release_kernel<kMaxRequests / kPlanThreads><<<dim3(1), dim3(kPlanThreads), 0, s>>>(a);
+  const int B = pool->requests;
+  constexpr int T = kPlanThreads, S = kSmallThreads;
+  if (B <= S) release_kernel<S, 1><<<dim3(1), dim3(S), 0, s>>>(a);
+  else if (B <= T) release_kernel<T, 1><<<dim3(1), dim3(T), 0, s>>>(a);
+  else if (B <= 2 * T) release_kernel<T, 2><<<dim3(1), dim3(T), 0, s>>>(a);
+  else release_kernel<T, kMaxRequests / T><<<dim3(1), dim3(T), 0, s>>>(a);
   FDLLM_RETURN_LAUNCH_STATUS(what);
 }
