@@ -227,11 +227,20 @@ __global__ __launch_bounds__(T) void assign_plan_kernel(const AssignArgs a, int 
 constexpr int kRowsPerWg = 256;  // with 1024 rows the searches of 16384 take 7.4 us in place of 4.2
 template <int N>  // at least as many requests
 __global__ __launch_bounds__(kRowsPerWg) void assign_rows_kernel(const AssignArgs a, int n_rows) {
-  __shared__ uint32_t s_end[N];
+  constexpr bool kAll = N <= kPlanThreads;  // what a request's rows need beside it: a round trip less
+  __shared__ uint32_t s_end[N], s_len[kAll ? N : 1];
+  __shared__ int32_t s_at[kAll ? N : 1];
   const fdllm_page_pool& p = a.pool;
   if (a.width == 0) {
-    for (int b = threadIdx.x; b < N; b += kRowsPerWg)
-      s_end[b] = static_cast<uint32_t>(a.row_starts[min(b + 1, p.requests)]);
+#pragma unroll 4
+    for (int k = 0; k < N; k += kRowsPerWg) {
+      const int b = threadIdx.x + k, c = min(b, p.requests - 1);
+      s_end[b] = static_cast<uint32_t>(a.row_starts[c + 1]);
+      if (kAll) {
+        s_len[b] = static_cast<uint32_t>(a.starts[c]) | (a.granted[c] > 0 ? 0x80000000u : 0);
+        s_at[b] = a.list_at[c];
+      }
+    }
     __syncthreads();
   }
   const int r = blockIdx.x * kRowsPerWg + threadIdx.x;
@@ -243,11 +252,12 @@ __global__ __launch_bounds__(kRowsPerWg) void assign_rows_kernel(const AssignArg
     if (t >= a.new_lens[b]) b = -1;
   } else {
     b = first_above<N>(s_end, static_cast<uint32_t>(r));
-    t = b < p.requests ? r - a.row_starts[b] : 0;
+    t = b > 0 ? r - static_cast<int>(s_end[min(b, N) - 1]) : r;  // begins are at most r: no saturation
     if (b >= p.requests) b = -1;
   }
-  if (b >= 0) put_row(a, r, b, t, static_cast<uint32_t>(a.starts[b]), a.granted[b] > 0, a.list_at[b]);
-  else put_row(a, r, -1, 0, 0, false, 0);
+  if (b < 0) put_row(a, r, -1, 0, 0, false, 0);
+  else if (kAll && a.width == 0) put_row(a, r, b, t, s_len[b] & 0x7fffffffu, s_len[b] >> 31, s_at[b]);
+  else put_row(a, r, b, t, static_cast<uint32_t>(a.starts[b]), a.granted[b] > 0, a.list_at[b]);
 }
 
 // keep_lens: pages behind the kept lengths go back, the last ones first.
