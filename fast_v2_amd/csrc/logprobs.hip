@@ -25,6 +25,8 @@
 // us, 16 x 8 bf16 rows with 5 15.4 us, of which the finish is 5: states and maxima 0.9 us, bound 1.1, groups 0.3, their
 // logits 0.9, ranks 0.5, launch. Its code runs once a row and is loaded for it, so it is kept
 // short: with loops unrolled the finish took 9 us (K = 5) to 19 (K = 20).
+#include <type_traits>
+
 #include "fdllm_common.h"
 
 namespace fdllm {
@@ -388,34 +390,40 @@ __device__ __forceinline__ void finish(const ScoreArgs& a, int64_t r, const RowV
   }
 }
 
+// The maximum of a value and another lane's, by a lane move within rows of 16.
+template <int CTRL>
+__device__ __forceinline__ float max_moved(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
+
 // The maximum over the lanes of each of the U values m[u], the u-th group's: where it is, value u of the
 // wave's U / 4 to a lane. Lanes trade halves of their values for halves of the others', so that two and
 // a few exchanges serve all.
 template <int U>
-__device__ __forceinline__ void group_maxima(float* m, int lane) {
-  const bool up32 = (lane & 32) != 0, up16 = (lane & 16) != 0;
+__device__ __forceinline__ void group_maxima(float* m) {
 #pragma unroll
-  for (int u = 0; u < U / 2; ++u) {
-    const float give = up32 ? m[u] : m[u + U / 2], own = up32 ? m[u + U / 2] : m[u];
-    m[u] = fmaxf(own, __shfl_xor(give, 32, kWave));
+  for (int u = 0; u < U / 2; ++u) {  // the upper 32 lanes take the second half's values
+    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(m[u]), __float_as_uint(m[u + U / 2]), false, false);
+    m[u] = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
   }
 #pragma unroll
-  for (int u = 0; u < U / 4; ++u) {
-    const float give = up16 ? m[u] : m[u + U / 4], own = up16 ? m[u + U / 4] : m[u];
-    m[u] = fmaxf(own, __shfl_xor(give, 16, kWave));
-    m[u] = fmaxf(m[u], dpp_f32<0xB1>(m[u]));
-    m[u] = fmaxf(m[u], dpp_f32<0x4E>(m[u]));
-    m[u] = fmaxf(m[u], dpp_f32<0x141>(m[u]));
-    m[u] = fmaxf(m[u], dpp_f32<0x140>(m[u]));
+  for (int u = 0; u < U / 4; ++u) {  // odd rows of 16 lanes the second half's of those
+    const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(m[u]), __float_as_uint(m[u + U / 4]), false, false);
+    m[u] = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    m[u] = max_moved<0xB1>(m[u]);
+    m[u] = max_moved<0x4E>(m[u]);
+    m[u] = max_moved<0x141>(m[u]);
+    m[u] = max_moved<0x140>(m[u]);
   }
 }
 
-// One workgroup per row, or per `steps` steps of a row that several share.
-template <typename T>
+// One workgroup per row, or (SPLIT) per `steps` steps of a row that several share; the latter without the
+// finish's LDS and code.
+template <typename T, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
   constexpr int N = Vec<T>::N, U = kStep / kWaves / Vec<T>::kGroup;  // a lane's vectors in a step
-  __shared__ Shared<T, kThreads> sh;
-  const uint32_t row = blockIdx.x / static_cast<uint32_t>(a.splits);
+  __shared__ std::conditional_t<SPLIT, char, Shared<T, kThreads>> sh;
+  const uint32_t row = SPLIT ? blockIdx.x / static_cast<uint32_t>(a.splits) : blockIdx.x;
   const int split = static_cast<int>(blockIdx.x - row * a.splits);
   const int64_t r = row;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -423,7 +431,7 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
   float* groups = a.parts + a.rows * a.splits * (4 * kWaves) + r * a.n_groups;  // splits > 1
   State st{-INFINITY, 0.f, 0.f};
   Given given{false, 0.f};
-  if (a.splits == 1) given = given_of<T>(a, r, threadIdx.x, rv);
+  if constexpr (!SPLIT) given = given_of<T>(a, r, threadIdx.x, rv);
 #pragma unroll 1
   for (int k = 0; k < a.steps; ++k) {
     const int g = ((split * a.steps + k) * kWaves + wave) * U;
@@ -477,20 +485,20 @@ __global__ __launch_bounds__(kThreads) void score_kernel(const ScoreArgs a) {
         }
     }
     if (a.top > 0) {
-      group_maxima<U>(mu, lane);
+      group_maxima<U>(mu);
       const int u0 = (lane >> 5) * (U / 2) + ((lane >> 4) & 1) * (U / 4);
       if ((lane & 15) == 0) {
 #pragma unroll
         for (int u = 0; u < U / 4; ++u)
           if (g + u0 + u < a.n_groups) {
-            if (a.splits > 1) groups[g + u0 + u] = mu[u];
+            if constexpr (SPLIT) groups[g + u0 + u] = mu[u];
             else sh.group[g + u0 + u] = mu[u];
           }
       }
     }
   }
   st = join_wave(st);
-  if (a.splits == 1) {
+  if constexpr (!SPLIT) {
     st = join<kWaves>(st, sh.red);  // a barrier: the group maxima are in LDS after it
     if (a.top > 0) {
       if (wave == 0) find_bound<T, kThreads>(a, lane, sh);
@@ -564,8 +572,13 @@ Cut cut(int vocab, int64_t rows, int dtype) {
 
 template <typename T>
 void launch(const ScoreArgs& a, hipStream_t s) {
-  score_kernel<T><<<dim3(static_cast<unsigned>(a.rows * a.splits)), dim3(kThreads), 0, s>>>(a);
-  if (a.splits > 1) score_finish_kernel<T><<<dim3(static_cast<unsigned>(a.rows)), dim3(kFinishThreads), 0, s>>>(a);
+  const dim3 grid(static_cast<unsigned>(a.rows * a.splits)), block(kThreads);
+  if (a.splits == 1) {
+    score_kernel<T, false><<<grid, block, 0, s>>>(a);
+  } else {
+    score_kernel<T, true><<<grid, block, 0, s>>>(a);
+    score_finish_kernel<T><<<dim3(static_cast<unsigned>(a.rows)), dim3(kFinishThreads), 0, s>>>(a);
+  }
 }
 
 int check_sizes(const char* what, int vocab, int64_t rows, int dtype) {
