@@ -235,7 +235,7 @@ __device__ __forceinline__ void find_bound(const ScoreArgs& a, int lane, Shared<
   sh.lane_max[lane] = mine;
   wave_sync();
   int above = 0;
-#pragma unroll 2
+#pragma unroll
   for (int h = 0; h < 64; h += 4) {
     const f32x4 y = *reinterpret_cast<const f32x4*>(&sh.lane_max[h]);
 #pragma unroll
@@ -523,8 +523,14 @@ __global__ __launch_bounds__(kFinishThreads) void score_finish_kernel(const Scor
   float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
   if (tid >> 6 == 1 && lane < np) p = parts[lane];
   if (a.top > 0) {
+    // two in flight
 #pragma unroll 1
-    for (int g = tid; g < a.n_groups; g += kFinishThreads) sh.group[g] = groups[g];
+    for (int g = tid; g < a.n_groups; g += 2 * kFinishThreads) {
+      const int h = g + kFinishThreads;
+      const float x = groups[g], y = h < a.n_groups ? groups[h] : -INFINITY;
+      sh.group[g] = x;
+      if (h < a.n_groups) sh.group[h] = y;
+    }
   }
   const Given given = given_of<T>(a, r, tid, rv);
   __syncthreads();
