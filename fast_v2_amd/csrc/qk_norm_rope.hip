@@ -103,12 +103,15 @@ struct NormRopeArgs {
 constexpr int kMaxDim = 256;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-// Tokens from which a wave takes a whole one; below, a workgroup's waves share a token (its angles
-// are computed once), with other workgroups while there are at most kResident waves. us, shared /
-// a wave each, bf16, 28 + 4 + 4 heads of 128: 1 token 3.4 / 7.3, 128 tokens 4.1 / 8.3, 600 6.2 /
-// 8.9, 1501 10.3 / 11.6, 2048 13.8 / 12.4, 16384 76 / 61. More waves a token, fp32, 12 + 2 + 2
-// heads (eight / four): 128 tokens 3.8 / 3.9, 314 4.7 / 4.4, 600 7.7 / 5.3.
-constexpr int kTokenPerWave = 2048;
+// Tokens from which a wave takes a whole one. Below, a workgroup's four waves share a token (its angles
+// are computed once), with other workgroups while there are at most kResident waves; from kPairTokens on two
+// waves share one, which is less code to issue in all and fills the machine no less. us, four / two waves / one:
+//   bf16, 28 + 4 + 4 heads of 128: 1 token 3.4 / - / 7.3, 128 4.1 / - / 8.3, 1000 7.1 / 8.0 / -,
+//     1501 10.3 / 9.4 / 11.6, 2048 13.8 / 10.9 / 12.8, 3000 - / 15.4 / 14.4
+//   fp32, 12 + 2 + 2 heads of 128: 1000 6.6 / 6.7 / -, 1501 9.7 / 8.8 / -, 2048 - / 10.7 / 10.9, 3000 - / 15.2 / 14.6
+// More waves a token, the latter (eight / four): 128 tokens 3.8 / 3.9, 314 4.7 / 4.4, 600 7.7 / 5.3.
+constexpr int kTokenPerWave = 2560;
+constexpr int kPairTokens = 1280;
 constexpr int kResident = 2048;
 constexpr int kAhead = 2;  // a wave's steps in flight
 constexpr int kMaxTokens = (1 << 25) - 1;  // a launch has fewer than 2^32 threads, a token 64, and workgroups are whole
@@ -151,7 +154,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeArgs 
   __shared__ __attribute__((aligned(16))) float s_c[kWaves][2][W], s_s[kWaves][2][W];
   __shared__ __attribute__((aligned(16))) float s_rows[LAY == kHalfLds ? kWaves : 1][LAY == kHalfLds ? 64 * 8 : 1];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  // A wave takes a whole token (parts 1), or a workgroup's waves, and those of others, share one. 32-bit
+  // A wave takes a whole token (parts 1), two share one, or a workgroup's waves, and those of others, do. 32-bit
   // divisions: there are fewer than 2^31 tokens, and a token has parts only where there are few
   const uint32_t job = blockIdx.x * kWaves + wave;
   const uint32_t row = min(job / static_cast<uint32_t>(a.parts), a.tokens - 1);
@@ -190,7 +193,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(const NormRopeArgs 
 
   // the tables, while the rows are in flight. Weights are read as whole words and taken apart
   // later: a conversion beside each load would wait for them one after another
-  const int at = a.parts > 1 ? threadIdx.x : lane, by = a.parts > 1 ? kThreads : 64, tab = a.parts > 1 ? 0 : wave;
+  // (parts is 1, 2 or a multiple of kWaves)
+  const int by = 64 * min(a.parts, kWaves), at = threadIdx.x & (by - 1), tab = a.parts == 1 ? wave : a.parts == 2 ? wave >> 1 : 0;
   const bool wide = d.weight_dtype == FDLLM_DTYPE_F32;
   const void* const wq = d.q_weight ? d.q_weight : d.k_weight;
   const void* const wk = d.k_weight ? d.k_weight : d.q_weight;
@@ -322,7 +326,9 @@ void launch(NormRopeArgs a, Layout lay, int64_t tokens, hipStream_t s) {
   a.k_steps = (a.d.num_kv_heads + HPS - 1) / HPS;
   const int all = a.all_steps = a.q_steps + (a.d.k_cache ? 2 : 1) * a.k_steps;  // value heads only go to the cache
   a.parts = 1;
-  if (tokens < kTokenPerWave) {
+  if (tokens < kTokenPerWave && tokens >= kPairTokens) {
+    a.parts = 2;
+  } else if (tokens < kTokenPerWave) {
     a.parts = (all + kWaves - 1) / kWaves * kWaves;
     while (a.parts > kWaves && tokens * a.parts > kResident) a.parts -= kWaves;
   }

@@ -100,6 +100,14 @@ def test_against_float64(gpu, case, dtype):
         assert torch.equal(c.reshape(pages * page, Hkv, D), want)
 
 
+@pytest.mark.parametrize("heads", [(3, 1, 128, 128, False), (9, 2, 80, 20, False), (2, 2, 64, 64, True), (5, 3, 256, 64, False)])
+@pytest.mark.parametrize("B,S", [(1, 600), (3, 427), (1, 1279), (1, 1281), (2, 1279), (1, 2559), (1, 2561), (7, 400)])
+def test_token_counts(gpu, B, S, heads):
+    """Several workgroups, waves, two waves and one wave to a token, with waves left over."""
+    Hq, Hkv, D, R, inter = heads
+    test_against_float64(gpu, (B, S, Hq, Hkv, D, R, inter, True, True, False), BF16 if S % 2 else F32)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_far_positions(gpu, dtype):
     """The angles of positions up to the type's end, and negative ones."""
