@@ -18,11 +18,11 @@
 // values, then the logits above it are ranked and its first equals fill up.
 //
 // What bounds it: many rows, the one read of the logits beside the vector units: 4 x 512 rows of 152064
-// bf16 logits (623 MB) 112 us, 5.6 TB/s, where a plain read of the memory takes 99. 9.6 vector instructions
-// a logit, one of them the exponential, are about 95 us of every SIMD (with edge checks in every step
+// bf16 logits (623 MB) 112 us, 5.6 TB/s, where a plain read of the memory takes 99. 9.2 vector instructions
+// a logit, one of them the exponential, are about 90 us of every SIMD (with edge checks in every step
 // and (x - m) log2 e as two operations 12 a logit and 117 us). The next step's loads ahead of this one's
-// arithmetic took 4 us more, as fewer waves fit. Few rows, latency: one fp32 row with 20 alternatives 9.5
-// us, 16 x 8 bf16 rows with 5 15.4 us, of which the finish is 5: states and maxima 0.9 us, bound 1.1, groups 0.3, their
+// arithmetic took 4 us more, as fewer waves fit. Few rows, latency: one fp32 row with 20 alternatives 8.9
+// us, 16 x 8 bf16 rows with 5 15.0 us, of which the finish is 5: states and maxima 0.9 us, bound 0.9, groups 0.3, their
 // logits 0.9, ranks 0.5, launch. Its code runs once a row and is loaded for it, so it is kept
 // short: with loops unrolled the finish took 9 us (K = 5) to 19 (K = 20).
 #include <type_traits>

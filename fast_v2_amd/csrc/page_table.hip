@@ -224,7 +224,7 @@ __global__ __launch_bounds__(T) void assign_plan_kernel(const AssignArgs a, int 
 }
 
 // The rows' part by itself, after the plan: their begins in LDS where they have to be searched.
-constexpr int kRowsPerWg = 256;  // with 1024 rows the searches of 16384 take 7.4 us in place of 4.2
+constexpr int kRowsPerWg = 256;  // with 1024 rows the searches of 16384 took 7.4 us in place of 4.2
 template <int N>  // at least as many requests
 __global__ __launch_bounds__(kRowsPerWg) void assign_rows_kernel(const AssignArgs a, int n_rows) {
   constexpr bool kAll = N <= kPlanThreads;  // what a request's rows need beside it: a round trip less

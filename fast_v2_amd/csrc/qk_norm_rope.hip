@@ -23,7 +23,7 @@
 // they stay). Few tokens, latency: one token 3.4 us, 16 x 8 4.1 us, of which an empty kernel is
 // 1.5: arguments, position and slot, rows and weights, stores. A workgroup for every token with a
 // barrier before its heads took 140 us for the large call; angles per wave with weights read
-// and converted one by one 66 us, and 8.2 us for 1501 packed tokens (7.0).
+// and converted one by one 66 us, and 8.2 us for 1501 packed tokens (6.5 with two waves for each).
 #include <algorithm>
 
 #include "fdllm_common.h"

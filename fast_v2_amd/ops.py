@@ -980,7 +980,8 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, page_table: torch.T
     few pages, only requests with room on their last page are served. ``slots`` and
     ``positions`` go to ``norm_rope_kv_write``, ``seqlens`` (and ``starts`` as ``q_start``) with
     the table to ``block_attn``. page_size is a power of two; at most 8192 requests. Changes
-    ``lens``, ``page_table`` and ``free_count`` in place: calls on one pool run in stream order.
+    ``lens``, ``page_table`` and ``free_count`` in place: calls on one pool run in stream order,
+    its tensors lie apart, and a page is one request's.
     """
     what = "assign_pages"
     if new_lens.is_cuda:

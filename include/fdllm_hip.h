@@ -499,7 +499,8 @@ int fdllm_unmask_step_ws(const void* logits, int64_t logits_stride_b, int64_t lo
  * tokens in each request's cache; negative counts as 0), and the free list: page ids
  * free_pages[0 .. *free_count), of which the last is handed out first. page_size is a power of
  * two (fdllm_kv_attn_fwd takes 16 and more). All int32. The calls below change the pool in
- * place, in stream order; calls on one pool must not overlap.
+ * place, in stream order; calls on one pool must not overlap, its arrays lie apart (from the
+ * calls' other arguments too), and a page is one request's: there are no reference counts.
  *
  * fdllm_assign_pages: request b asks for new_lens[b] tokens (none where it is not positive).
  *   Its rows: width > 0 (padded form): rows b * width .. + width - 1 of [requests, width];
