@@ -25,6 +25,7 @@
 // us, 16 x 8 bf16 rows with 5 15.0 us, of which the finish is 5: states and maxima 0.9 us, bound 0.9, groups 0.3, their
 // logits 0.9, ranks 0.5, launch. Its code runs once a row and is loaded for it, so it is kept
 // short: with loops unrolled the finish took 9 us (K = 5) to 19 (K = 20).
+#include <algorithm>
 #include <type_traits>
 
 #include "fdllm_common.h"
@@ -37,8 +38,8 @@ constexpr int kWaves = kThreads / 64;
 // Threads of a row's finish: 256 take 0.9 us more for 20 alternatives of one fp32 row, 1024 1.3 us
 // more (2 to 5 us where there are many rows).
 constexpr int kFinishThreads = 512;
-// Workgroups that a call aims at: 1024 take 1.8 us more for 16 x 8 rows of 152064, 4096 0.9 us more (more
-// partials, one step each); from 2048 rows on a workgroup takes whole rows.
+// Workgroups that a call aims at where rows are shared: 1024 take 1.8 us more for 16 x 8 rows of 152064, 4096
+// 0.9 us more (more partials, one step each).
 constexpr int kWorkgroups = 2048;
 constexpr int kStep = 2048 * kWaves;      // logits of a workgroup's step
 constexpr int kMaxVocab = 1 << 20;
@@ -561,15 +562,18 @@ struct Cut {
   int n_groups, steps, splits;
   size_t bytes;
 };
-// Rows are shared by workgroups until there are kWorkgroups of them.
+// A workgroup takes a whole row where it has at most two steps, and where there are many rows (a finish less, and
+// no partials); else several share one. us, bf16, whole rows / shared: 9000 logits, 16 rows 8.7 / 8.8, 500
+// 9.2 / 10.9, 1000 11.1 / 15.2; 32000, 16 rows 9.8 / 8.6, 333 13.2 / 12.0, 500 14.1 / 15.0, 1000 19.4 / 22.7;
+// 152064, 333 37.6 / 27.8, 500 39.2 / 36.5, 600 45.6 / 43.4, 850 56.6 / 59.8, 1000 60.8 / 65.
 Cut cut(int vocab, int64_t rows, int dtype) {
   Cut c;
   const int slack = dtype == FDLLM_DTYPE_F32 ? 3 : 7;  // a row may start inside a vector
   const int group = dtype == FDLLM_DTYPE_F32 ? Vec<float>::kGroup : Vec<bf16_t>::kGroup;
   c.n_groups = (vocab + slack + group - 1) / group;
   const int64_t all = (static_cast<int64_t>(c.n_groups) * group + kStep - 1) / kStep;
-  const int64_t want = rows < kWorkgroups ? kWorkgroups / rows : 1;
-  const int64_t splits = want < all ? want : all;
+  const bool whole = all <= 2 || rows >= (all <= 4 ? 448 : 640);
+  const int64_t splits = whole ? 1 : std::min<int64_t>(kWorkgroups / rows, all);
   c.steps = static_cast<int>((all + splits - 1) / splits);
   c.splits = static_cast<int>((all + c.steps - 1) / c.steps);
   c.bytes = c.splits > 1 ? (static_cast<size_t>(rows) * c.splits * (4 * kWaves) + static_cast<size_t>(rows) * c.n_groups) * 4 : 0;

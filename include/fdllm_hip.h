@@ -603,7 +603,7 @@ int fdllm_norm_rope_kv_write(const fdllm_norm_rope_kv_desc* desc, void* stream);
  * in fp32; all outputs contiguous. A row without a distribution (it holds NaN or +inf, or
  * nothing above -inf) gives NaN, and -1 for top_tokens.
  *
- * `workspace` (fdllm_token_logprobs_workspace_size bytes, 0 for many rows; 16-byte aligned)
+ * `workspace` (fdllm_token_logprobs_workspace_size bytes, 0 where no row is shared; 16-byte aligned)
  * needs no initialisation; calls that may overlap in time need separate ones. One kernel, or two
  * where workgroups share a row. vocab is at most 2^20 - 8, and there are fewer than 2^24 rows.
  *

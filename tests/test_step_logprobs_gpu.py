@@ -75,6 +75,29 @@ def test_row_counts(gpu, rows, V, dtype):
     _check(x, torch.arange(rows, device=gpu) % V, min(V, 8))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,V", [(1, 16384), (1, 16385), (2, 16392), (5, 24571), (447, 20001), (448, 20001), (447, 33001),
+                                    (640, 33001)])
+def test_shared_and_whole_rows(gpu, rows, V, dtype):
+    """On either side of the rule by which workgroups share rows; every second row starts inside a vector."""
+    print(f"case logprobs shared {rows}x{V} {dtype}", flush=True)
+    x = _randn(gpu, (rows, V + 1), dtype, rows + V)[:, 1:]
+    tokens = torch.arange(3 * rows, device=gpu).view(rows, 3) * 1001 % V
+    _check(x, tokens, 20, (rows, V))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("V", [20011, 152064])
+def test_orders_of_shared_rows(gpu, V, dtype):
+    print(f"case logprobs orders V={V} {dtype}", flush=True)
+    at = torch.arange(V, device=gpu)
+    up = at.float() * (60.0 / V)
+    x = torch.stack([up, up.flip(0), torch.zeros_like(up), (at % 7).float(), torch.where(at == V - 3, 9.0, 1.0), up.round(),
+                     -up * 100, torch.where(at % 1000 == 999, 5.0, -float("inf"))])
+    for k in (1, 20, 32):
+        _check(x.to(dtype), torch.full((len(x),), 999, device=gpu), k, (V, dtype, k))
+
+
 @pytest.mark.parametrize("rows", [3, 2200])
 def test_orders(gpu, rows):
     """Ties, sorted and constant rows: the alternatives' worst cases."""
